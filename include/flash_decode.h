@@ -514,6 +514,131 @@ FD_API int fd_kv_append(void* stream, const void* k_new, const void* v_new, void
                  int64_t stride_v_tok, int64_t stride_v_h,
                  int64_t stride_table_bs, const fd_qk_prep* prep, const fd_params* params);
 
+/*
+ * Attention of many query rows per sequence: whole prompts, chunks of prompts behind what the cache holds, drafted
+ * tokens (the step that the reference's attention block makes for more than one new token,
+ * python/triton_dist/layers/amd/tp_attn.py:262-269).
+ *
+ *  q            [total_q, Hq, D]          sequence b's rows are cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1
+ *  keys, packed [total_k, Hkv, D]         (block_table NULL) sequence b's keys are cu_seqlens_k[b] .. [b + 1] - 1
+ *  keys, paged  [num_pages, P, Hkv, D]    (block_table given) kv_lens[b] tokens, new ones included
+ *  x[i, j] = sm_scale * q_i . k_j, soft-capped if params.soft_cap > 0; row i of n_q sees the keys j < n_k and, causal,
+ *  j <= i + n_k - n_q: the last row sees the last key, whatever the lengths.  A row that sees nothing gets out = 0,
+ *  lse = -inf.  Rows that belong to no sequence (behind the last one, before the first, behind q_lens[b]) are left as
+ *  they are.  What lies behind a sequence's last key is not read.
+ *  No device value can lead a kernel out of bounds: offsets, lengths and page ids are clamped.
+ */
+typedef struct fd_prefill_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;                  /* [total_q, Hq, D] in the query's type                                                */
+  float* lse_out;             /* NULL or fp32 [total_q, Hq]: natural-log LSE                                         */
+  void* workspace;            /* fd_prefill_workspace_bytes(...) bytes on a 256-byte boundary (NULL where that is 0)  */
+  int64_t workspace_bytes;
+  const int32_t* cu_seqlens_q;/* [batch + 1]; NULL with batch 1: all rows                                            */
+  const int32_t* q_lens;      /* NULL, or [batch]: only the first q_lens[b] rows of sequence b are real (padded batch)*/
+  const int32_t* cu_seqlens_k;/* packed keys: [batch + 1]                                                            */
+  const int32_t* kv_lens;     /* paged keys: [batch]                                                                 */
+  const int32_t* block_table; /* NULL: packed keys                                                                   */
+  int64_t stride_q_t, stride_q_h, stride_k_tok, stride_k_h, stride_v_tok, stride_v_h;
+  int64_t stride_ot, stride_oh, stride_table_bs;
+  float sm_scale;
+  int32_t batch, total_q;
+  int32_t total_k;            /* packed keys: rows of k and v                                                        */
+  int32_t causal;
+  fd_params params;           /* q_heads, kv_heads, head_dim, page_size, num_pages, max_pages_per_seq, q_dtype (16-bit),
+                                 kv_dtype (the query's, or FD_FP8_E4M3 with k_scale / v_scale and a block table),
+                                 soft_cap, max_kv_len (hint); num_splits: 0 = the library chooses, else exactly that
+                                 many key ranges per row tile                                                        */
+} fd_prefill_args;
+
+/* Bytes of workspace that fd_prefill needs for these arguments (the partials of split key ranges), or a negative
+ * fd_status.  Reads sizes, types and params only. */
+FD_API int64_t fd_prefill_workspace_bytes(const fd_prefill_args* args);
+
+FD_API int fd_prefill(void* stream, const fd_prefill_args* args);
+
+/*
+ * One decode step of sequences that share prefixes.  Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1;
+ * all of them attend to the prefix_lens[g] tokens of row g of prefix_table, and each of them to its own kv_lens[b] tokens
+ * of block_table behind that (0 is allowed, for either).  A prefix is read once for its group: its part is a matrix product
+ * of all the group's rows (fd_prefill's kernel), the sequences' own tokens go through the decode kernel, and one launch
+ * merges the partials of both by their LSEs.  A sequence outside every group attends to its own tokens only.
+ * `step` is the decode step over the sequences' own tokens as for fd_decode_planned, with combine_mode FD_COMBINE_SPLIT and
+ * without extra partials, seq_order and flags; its workspace is the whole step's (fd_decode_shared_workspace_bytes).
+ * 16-bit queries, caches of the same type or fp8, equal K and V head dims.
+ */
+typedef struct fd_shared_args {
+  fd_decode_args step;
+  const int32_t* prefix_table; /* [groups, prefix_max_pages]                                                         */
+  const int32_t* prefix_lens;  /* [groups]                                                                           */
+  const int32_t* group_starts; /* [groups + 1]; NULL with one group: all sequences                                   */
+  int64_t stride_prefix_bs;
+  int32_t groups, prefix_max_pages;
+  int32_t max_prefix_len;      /* 0, or an upper bound of prefix_lens known on the host (a hint, like max_kv_len)    */
+} fd_shared_args;
+
+FD_API int64_t fd_decode_shared_workspace_bytes(const fd_shared_args* args);
+
+FD_API int fd_decode_shared(void* stream, const fd_shared_args* args);
+
+/*
+ * Pages of a cache.  The tables live on the device and nothing is read on the host: block_table rows hold their pages from
+ * the front and -1 behind them, page_refs counts the rows that hold a page (0: free).  A free page is handed out lowest id
+ * first, in the order of the requests: the same calls give the same tables.  Calls on one set of tables follow each other on
+ * one stream.
+ */
+typedef struct fd_page_pool {
+  void* k_cache;              /* [layers, num_pages, P, heads, dim]: a page is contiguous, 16-byte aligned, and a
+                                 multiple of 16 bytes per token                                                       */
+  void* v_cache;              /* same pages, its own strides and dims                                                 */
+  int64_t k_layer_stride, k_page_stride, k_page_bytes;   /* bytes                                                     */
+  int64_t v_layer_stride, v_page_stride, v_page_bytes;
+  int32_t layers, num_pages, page_size;
+} fd_page_pool;
+
+typedef struct fd_page_tables {
+  int32_t* block_table;       /* [batch, max_pages_per_seq]                                                           */
+  int32_t* kv_lens;           /* [batch]                                                                              */
+  int32_t* page_refs;         /* [num_pages]                                                                          */
+  int64_t stride_table_bs;
+  int32_t batch, max_pages_per_seq;
+} fd_page_tables;
+
+/* Page src_pages[i] to page dst_pages[i], in every layer of both pools.  The destinations are distinct and none of them is a
+ * source; ids outside the pool are skipped. */
+FD_API int fd_pages_copy(void* stream, const fd_page_pool* pool, const int32_t* src_pages, const int32_t* dst_pages,
+                         int32_t count);
+
+/* Gives row b the pages that kv_lens[b] + new_tokens[b] tokens need (new_tokens NULL: `uniform` for every row).  ok[b]: 1, or
+ * 0 where the table is too narrow or the pool has run out by then -- such a row keeps what it had.  Rows are served in
+ * order, and a row that gets nothing still counts against the rows behind it.  batch <= 4096. */
+FD_API int fd_pages_reserve(void* stream, const fd_page_tables* tables, int32_t num_pages, int32_t page_size,
+                            const int32_t* new_tokens, int32_t uniform, int32_t* ok);
+
+/* Makes row children[i] a fork of row parents[i]: same length, the parent's full pages shared (their counts go up), the
+ * tokens of a part-filled last page copied to a fresh page of its own in every layer, so that both rows can be appended
+ * to.  ok[i]: 1, or 0 where the fork is refused and nothing changes: a row out of range, a child that is its own parent, that
+ * holds tokens or pages or was named before in the list, no free page left.  Parents count as they are before the call.
+ * workspace: fd_pages_workspace_bytes(num_pages, count) bytes. */
+FD_API int fd_pages_fork(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, const int32_t* parents,
+                         const int32_t* children, int32_t count, int32_t* ok, void* workspace, int64_t workspace_bytes);
+
+/* Takes the listed rows' pages from them (counts go down, entries become -1) and sets their lengths to 0.  Rows that hold
+ * nothing, are listed twice or lie out of range are skipped. */
+FD_API int fd_pages_free(void* stream, const fd_page_tables* tables, int32_t num_pages, const int32_t* rows,
+                         int32_t count);
+
+/* Moves the live pages to the front of the pool: with n live pages, the k-th live page at or behind n goes to the k-th free
+ * page before n, in every layer, counts and tables with it.  *live_out (device): n.  `tables` must hold every row that holds
+ * pages. */
+FD_API int fd_pages_compact(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, int32_t* live_out,
+                            void* workspace, int64_t workspace_bytes);
+
+/* Workspace of fd_pages_fork (count forks) and fd_pages_compact (count 0), on a 16-byte boundary. */
+FD_API int64_t fd_pages_workspace_bytes(int32_t num_pages, int32_t count);
+
 /* Message for the last non-zero status returned on this thread ("" if none). */
 FD_API const char* fd_last_error(void);
 

@@ -31,7 +31,9 @@ FD_STEP_CALLER_PARTIALS, FD_STEP_ORDER_FROM_APPEND = 32, 64
 FD_ORDER_NONE, FD_ORDER_SEQUENCES, FD_ORDER_ITEMS = 0, 1, 2
 
 EXPORTED_SYMBOLS = ("fd_split_kv", "fd_combine", "fd_decode", "fd_plan_decode", "fd_workspace_bytes", "fd_decode_planned", "fd_decode_noalloc", "fd_schedule", "fd_schedule_items", "fd_plan_splits", "fd_plan_min_splits",
-                    "fd_kv_append",
+                    "fd_kv_append", "fd_prefill", "fd_prefill_workspace_bytes", "fd_decode_shared",
+                    "fd_decode_shared_workspace_bytes", "fd_pages_copy", "fd_pages_reserve", "fd_pages_fork", "fd_pages_free",
+                    "fd_pages_compact", "fd_pages_workspace_bytes",
                     "fd_last_error", "fd_abi_version", "fd_build_id")
 
 _DTYPES = {torch.float32: FD_F32, torch.float16: FD_F16, torch.bfloat16: FD_BF16}
@@ -110,6 +112,44 @@ class FdQkPrep(Structure):
     ]
 
 
+class FdPrefillArgs(Structure):
+    """Mirror of ``struct fd_prefill_args``."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse_out", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64), ("cu_seqlens_q", c_void_p), ("q_lens", c_void_p),
+        ("cu_seqlens_k", c_void_p), ("kv_lens", c_void_p), ("block_table", c_void_p),
+        ("stride_q_t", c_int64), ("stride_q_h", c_int64), ("stride_k_tok", c_int64), ("stride_k_h", c_int64),
+        ("stride_v_tok", c_int64), ("stride_v_h", c_int64), ("stride_ot", c_int64), ("stride_oh", c_int64),
+        ("stride_table_bs", c_int64), ("sm_scale", c_float), ("batch", c_int32), ("total_q", c_int32),
+        ("total_k", c_int32), ("causal", c_int32), ("params", FdParams),
+    ]
+
+
+class FdSharedArgs(Structure):
+    """Mirror of ``struct fd_shared_args``."""
+    _fields_ = [
+        ("step", FdDecodeArgs), ("prefix_table", c_void_p), ("prefix_lens", c_void_p), ("group_starts", c_void_p),
+        ("stride_prefix_bs", c_int64), ("groups", c_int32), ("prefix_max_pages", c_int32), ("max_prefix_len", c_int32),
+    ]
+
+
+class FdPagePool(Structure):
+    """Mirror of ``struct fd_page_pool``."""
+    _fields_ = [
+        ("k_cache", c_void_p), ("v_cache", c_void_p), ("k_layer_stride", c_int64), ("k_page_stride", c_int64),
+        ("k_page_bytes", c_int64), ("v_layer_stride", c_int64), ("v_page_stride", c_int64), ("v_page_bytes", c_int64),
+        ("layers", c_int32), ("num_pages", c_int32), ("page_size", c_int32),
+    ]
+
+
+class FdPageTables(Structure):
+    """Mirror of ``struct fd_page_tables``."""
+    _fields_ = [
+        ("block_table", c_void_p), ("kv_lens", c_void_p), ("page_refs", c_void_p), ("stride_table_bs", c_int64),
+        ("batch", c_int32), ("max_pages_per_seq", c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -163,6 +203,27 @@ def load_library(path: str = None) -> ctypes.CDLL:
         i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, POINTER(FdQkPrep), POINTER(FdParams)]
     lib.fd_schedule.restype = c_int32
     lib.fd_schedule.argtypes = [c_void_p, c_void_p, c_int32, c_void_p]
+    lib.fd_prefill.restype = c_int32
+    lib.fd_prefill.argtypes = [c_void_p, POINTER(FdPrefillArgs)]
+    lib.fd_prefill_workspace_bytes.restype = c_int64
+    lib.fd_prefill_workspace_bytes.argtypes = [POINTER(FdPrefillArgs)]
+    lib.fd_decode_shared.restype = c_int32
+    lib.fd_decode_shared.argtypes = [c_void_p, POINTER(FdSharedArgs)]
+    lib.fd_decode_shared_workspace_bytes.restype = c_int64
+    lib.fd_decode_shared_workspace_bytes.argtypes = [POINTER(FdSharedArgs)]
+    pool, tables = POINTER(FdPagePool), POINTER(FdPageTables)
+    lib.fd_pages_copy.restype = c_int32
+    lib.fd_pages_copy.argtypes = [c_void_p, pool, c_void_p, c_void_p, c_int32]
+    lib.fd_pages_reserve.restype = c_int32
+    lib.fd_pages_reserve.argtypes = [c_void_p, tables, c_int32, c_int32, c_void_p, c_int32, c_void_p]
+    lib.fd_pages_fork.restype = c_int32
+    lib.fd_pages_fork.argtypes = [c_void_p, pool, tables, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64]
+    lib.fd_pages_free.restype = c_int32
+    lib.fd_pages_free.argtypes = [c_void_p, tables, c_int32, c_void_p, c_int32]
+    lib.fd_pages_compact.restype = c_int32
+    lib.fd_pages_compact.argtypes = [c_void_p, pool, tables, c_void_p, c_void_p, c_int64]
+    lib.fd_pages_workspace_bytes.restype = c_int64
+    lib.fd_pages_workspace_bytes.argtypes = [c_int32, c_int32]
     lib.fd_last_error.restype = c_char_p
     lib.fd_last_error.argtypes = []
     lib.fd_abi_version.restype = c_int32

@@ -1198,4 +1198,410 @@ int fd_decode_planned(void* stream, const fd_decode_args* a) {
                    a->combine_mode, a->extra_out, a->extra_lse, a->num_extra, nullptr, &sp.p);
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Attention of many query rows (fd_prefill) and the shared-prefix decode step (fd_decode_shared).
+
+namespace {
+
+constexpr int kMaxPrefillSplits = 64;
+
+struct PrefillPlan {
+  int row_groups;             // 32-row groups of a workgroup's tile: 1, 2 or 4
+  int splits;                 // key ranges per row tile
+  int64_t part_bytes, lse_off, total;
+};
+
+// Row tile and key ranges from what the host knows: sizes, not lengths.  `rows` query rows (tokens) in `batch` sequences,
+// `tokens` keys in the longest.
+//  * Row tile: 128 rows of a KV head (token, head pairs) where a sequence has more than 64 on average; below that the waves
+//    of a workgroup share the keys of 64 or 32 rows instead of idling on rows that do not exist.
+//  * Key ranges: two workgroups fit a CU (one with head_dim 256); a grid that leaves half of those places empty is cut
+//    along the keys, as long as a range keeps four tiles, and the partials are merged by a second launch.
+void plan_prefill(const fd_params* p, int32_t batch, int64_t rows, int64_t tokens, int want_splits, PrefillPlan* pl) {
+  const int G = p->q_heads / p->kv_heads;
+  const int64_t avg = batch > 0 ? (rows * G + batch - 1) / batch : 0;
+  pl->row_groups = avg <= 32 && p->head_dim != 256 ? 1 : avg <= 64 ? 2 : 4;
+  const int bm = 32 * pl->row_groups;
+  const int bn = p->head_dim == 256 ? 32 : 64;
+  const int64_t places = p->head_dim == 256 ? 256 : 512;
+  int64_t tiles = (rows * G + bm - 1) / bm;
+  if (tiles < batch) tiles = batch;
+  int64_t s = want_splits;
+  if (s <= 0) {
+    s = 1;
+    const int64_t items = tiles * p->kv_heads;
+    if (items > 0 && 2 * items <= places) {
+      s = places / items;
+      const int64_t most = (tokens + bn - 1) / bn / 4;
+      if (s > most) s = most;
+      if (s > kMaxPrefillSplits) s = kMaxPrefillSplits;
+      if (s < 1) s = 1;
+    }
+  }
+  pl->splits = (int)s;
+  const int64_t lines = rows * p->q_heads * s;
+  pl->part_bytes = s > 1 ? lines * p->head_dim * 4 : 0;
+  pl->lse_off = align256(pl->part_bytes);
+  pl->total = s > 1 ? pl->lse_off + align256(lines * 4) : 0;
+}
+
+// Everything about a row-tile launch that does not depend on pointers.
+int check_prefill_shape(const char* fn, const fd_params* p, int32_t batch, int64_t rows, bool paged) {
+  if (batch < 0 || rows < 0) return fail(FD_ERR_INVALID_ARG, "%s: batch %d, %lld rows", fn, batch, (long long)rows);
+  if (p->q_heads <= 0 || p->kv_heads <= 0 || p->q_heads % p->kv_heads != 0)
+    return fail(FD_ERR_INVALID_ARG, "%s: q_heads %d must be a positive multiple of kv_heads %d", fn, p->q_heads,
+                p->kv_heads);
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(FD_ERR_UNSUPPORTED, "%s: head_dim %d (64/128/256)", fn, p->head_dim);
+  if (v_dim(p) != p->head_dim)
+    return fail(FD_ERR_UNSUPPORTED, "%s: K and V head dims must be equal (%d, %d)", fn, p->head_dim, v_dim(p));
+  if (p->q_dtype != FD_F16 && p->q_dtype != FD_BF16)
+    return fail(FD_ERR_UNSUPPORTED, "%s: q_dtype %d (fp16 or bf16)", fn, p->q_dtype);
+  if (p->kv_dtype != p->q_dtype && p->kv_dtype != FD_FP8_E4M3)
+    return fail(FD_ERR_UNSUPPORTED, "%s: kv_dtype %d (the query's type or fp8)", fn, p->kv_dtype);
+  if (p->kv_dtype == FD_FP8_E4M3 && !paged)
+    return fail(FD_ERR_UNSUPPORTED, "%s: fp8 keys are a cache's (paged) only", fn);
+  if (p->num_splits < 0 || p->num_splits > kMaxPrefillSplits)
+    return fail(FD_ERR_INVALID_ARG, "%s: num_splits %d (0: the library chooses, at most %d)", fn, p->num_splits,
+                kMaxPrefillSplits);
+  if (rows * p->q_heads >= (int64_t)1 << 31)
+    return fail(FD_ERR_TOO_LARGE, "%s: %lld query rows of %d heads", fn, (long long)rows, p->q_heads);
+  if (paged) {
+    if (p->page_size <= 0 || p->num_pages <= 0 || p->max_pages_per_seq <= 0)
+      return fail(FD_ERR_INVALID_ARG, "%s: page_size/num_pages/max_pages_per_seq must be > 0", fn);
+    if ((int64_t)p->num_pages * p->page_size >= (int64_t)1 << 31)
+      return fail(FD_ERR_TOO_LARGE, "%s: pool of %lld token rows exceeds 2^31", fn,
+                  (long long)p->num_pages * p->page_size);
+    if ((int64_t)p->max_pages_per_seq * p->page_size >= ((int64_t)1 << 31) - 256)
+      return fail(FD_ERR_TOO_LARGE, "%s: block table capacity exceeds 2^31 tokens", fn);
+  }
+  return FD_OK;
+}
+
+int check_prefill(const char* fn, const fd_prefill_args* a, PrefillPlan* pl) {
+  const fd_params* p = &a->params;
+  const bool paged = a->block_table != nullptr;
+  if (int rc = check_prefill_shape(fn, p, a->batch, a->total_q, paged)) return rc;
+  if (!paged && a->total_k < 0) return fail(FD_ERR_INVALID_ARG, "%s: total_k %d", fn, a->total_k);
+  // packed keys: the longest sequence is not known; all of them where there is one, else twice the average
+  int64_t tokens;
+  if (paged) {
+    tokens = planned_tokens(p);
+  } else {
+    tokens = a->batch > 1 ? 2 * ((int64_t)a->total_k / a->batch + 1) : a->total_k;
+    if (tokens > a->total_k) tokens = a->total_k;
+    if (p->max_kv_len > 0 && p->max_kv_len < tokens) tokens = p->max_kv_len;
+  }
+  plan_prefill(p, a->batch, a->total_q, tokens, p->num_splits, pl);
+  return FD_OK;
+}
+
+// Rows, keys and strides of a launch; pointers and alignment are checked here.
+int fill_prefill(const char* fn, const fd_prefill_args* a, PrefillArgs* k) {
+  const fd_params* p = &a->params;
+  if (!a->q || !a->k || !a->v || !a->out) return fail(FD_ERR_INVALID_ARG, "%s: NULL tensor pointer", fn);
+  if (!a->cu_seqlens_q && a->batch > 1)
+    return fail(FD_ERR_INVALID_ARG, "%s: %d sequences need their row offsets", fn, a->batch);
+  if (a->block_table ? !a->kv_lens : !a->cu_seqlens_k)
+    return fail(FD_ERR_INVALID_ARG, "%s: paged keys need kv_lens, packed keys cu_seqlens_k", fn);
+  const bool fp8 = p->kv_dtype == FD_FP8_E4M3;
+  if (fp8 && (!p->k_scale || !p->v_scale))
+    return fail(FD_ERR_INVALID_ARG, "%s: fp8 KV cache needs k_scale and v_scale", fn);
+  const int kv16 = fp8 ? 16 : 8;
+  if (!aligned16(a->q) || a->stride_q_t % 8 || a->stride_q_h % 8)
+    return fail(FD_ERR_ALIGNMENT, "%s: q rows must be 16-byte aligned (pointer and token/head strides)", fn);
+  if (!aligned16(a->k) || !aligned16(a->v) || a->stride_k_tok % kv16 || a->stride_k_h % kv16 ||
+      a->stride_v_tok % kv16 || a->stride_v_h % kv16)
+    return fail(FD_ERR_ALIGNMENT, "%s: K/V rows must be 16-byte aligned (pointer and token/head strides)", fn);
+  if ((reinterpret_cast<uintptr_t>(a->out) & 7) || a->stride_ot % 4 || a->stride_oh % 4)
+    return fail(FD_ERR_ALIGNMENT, "%s: output rows must be 8-byte aligned (pointer and token/head strides)", fn);
+  memset(k, 0, sizeof(*k));
+  k->q = a->q; k->k = a->k; k->v = a->v; k->out = a->out; k->lse = a->lse_out;
+  k->cu_q = a->cu_seqlens_q; k->q_lens = a->q_lens; k->cu_k = a->cu_seqlens_k; k->kv_lens = a->kv_lens;
+  k->bt = a->block_table; k->k_scale = p->k_scale; k->v_scale = p->v_scale;
+  k->sq_t = a->stride_q_t; k->sq_h = a->stride_q_h; k->sk_t = a->stride_k_tok; k->sk_h = a->stride_k_h;
+  k->sv_t = a->stride_v_tok; k->sv_h = a->stride_v_h; k->so_t = a->stride_ot; k->so_h = a->stride_oh;
+  k->sbt = a->stride_table_bs; k->sm_scale = a->sm_scale; k->soft_cap = p->soft_cap > 0.f ? p->soft_cap : 0.f;
+  k->batch = a->batch; k->total_q = a->total_q; k->total_k = a->total_k; k->Hq = p->q_heads; k->Hkv = p->kv_heads;
+  k->G = p->q_heads / p->kv_heads; k->P = a->block_table ? p->page_size : 1; k->max_pages = p->max_pages_per_seq;
+  k->num_pages = p->num_pages; k->causal = a->causal ? 1 : 0; k->splits = 1;
+  div_magic((uint32_t)k->P, &k->p_magic, &k->p_shift);
+  div_magic((uint32_t)k->G, &k->g_magic, &k->g_shift);
+  return FD_OK;
+}
+
+int launch_rows(const char* fn, void* stream, const PrefillArgs& k, const fd_params* p, int row_groups) {
+  const bool fp8 = p->kv_dtype == FD_FP8_E4M3;
+  auto launch = p->head_dim == 64 ? fd_launch_prefill_d64 : p->head_dim == 128 ? fd_launch_prefill_d128 : fd_launch_prefill_d256;
+  const int rc = launch((hipStream_t)stream, k, p->q_dtype, fp8, row_groups);
+  if (rc == FD_ERR_TOO_LARGE) return fail(rc, "%s: too many row tiles for one launch", fn);
+  if (rc != FD_OK) return fail(rc, "%s: launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
+  return FD_OK;
+}
+
+int check_workspace(const char* fn, const void* ws, int64_t have, int64_t need, uintptr_t align) {
+  if (need > 0 && (!ws || (reinterpret_cast<uintptr_t>(ws) & (align - 1)) || have < need))
+    return fail(FD_ERR_INVALID_ARG, "%s: needs a %d-byte aligned workspace of %lld bytes, got %p with %lld", fn,
+                (int)align, (long long)need, ws, (long long)have);
+  return FD_OK;
+}
+
+// Plan of a shared-prefix step: the decode step over the sequences' own tokens (fp32 partials, every slot written) and the
+// row tiles over the prefixes, one workspace for both.
+struct SharedPlan {
+  StepPlan step;
+  PrefillPlan rows;
+  fd_params prefix;
+  int64_t own_off, own_lse_off, order_off, total;
+};
+
+int plan_shared(const char* fn, const fd_shared_args* a, SharedPlan* sp) {
+  const fd_params* p = &a->step.params;
+  const int32_t batch = a->step.batch;
+  if (a->groups < 0 || (a->groups > 0 && a->prefix_max_pages <= 0))
+    return fail(FD_ERR_INVALID_ARG, "%s: groups %d, prefix_max_pages %d", fn, a->groups, a->prefix_max_pages);
+  if (a->step.flags || a->step.num_extra || a->step.seq_order || p->rank_merge ||
+      a->step.combine_mode != FD_COMBINE_SPLIT)
+    return fail(FD_ERR_INVALID_ARG, "%s: a step without flags, extra partials, order or rank merge, in FD_COMBINE_SPLIT", fn);
+  if (p->out_dtype != p->q_dtype) return fail(FD_ERR_UNSUPPORTED, "%s: the output has the query's type", fn);
+  sp->prefix = *p;
+  sp->prefix.max_pages_per_seq = a->prefix_max_pages > 0 ? a->prefix_max_pages : 1;
+  sp->prefix.max_kv_len = a->max_prefix_len;
+  sp->prefix.num_splits = 0;
+  if (int rc = check_prefill_shape(fn, &sp->prefix, batch, batch, true)) return rc;
+  if (int rc = plan_step(fn, p, batch, 1, 0, false, &sp->step)) return rc;
+  sp->step.p.mid_dtype = FD_F32;
+  const int64_t tokens = planned_tokens(&sp->prefix);
+  plan_prefill(&sp->prefix, a->groups, batch, tokens, 0, &sp->rows);
+  // the prefix part always leaves partials: there are the sequences' own to merge with
+  const int64_t lines = (int64_t)batch * p->q_heads;
+  const int D = p->head_dim;
+  sp->rows.part_bytes = lines * sp->rows.splits * D * 4;
+  sp->rows.lse_off = align256(sp->rows.part_bytes);
+  sp->own_off = sp->rows.lse_off + align256(lines * sp->rows.splits * 4);
+  const int64_t own = lines * sp->step.p.num_splits;
+  sp->own_lse_off = sp->own_off + align256(own * D * 4);
+  sp->order_off = sp->own_lse_off + align256(own * 4);
+  sp->total = sp->order_off + align256(sp->step.order_bytes);
+  return FD_OK;
+}
+
+}  // namespace
+
+int64_t fd_prefill_workspace_bytes(const fd_prefill_args* a) {
+  const char* fn = "fd_prefill_workspace_bytes";
+  if (!a) return fail(FD_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  PrefillPlan pl;
+  if (int rc = check_prefill(fn, a, &pl)) return rc;
+  return pl.total;
+}
+
+int fd_prefill(void* stream, const fd_prefill_args* a) {
+  const char* fn = "fd_prefill";
+  if (!a) return fail(FD_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  PrefillPlan pl;
+  if (int rc = check_prefill(fn, a, &pl)) return rc;
+  if (a->batch == 0 || a->total_q == 0) return FD_OK;
+  PrefillArgs k;
+  if (int rc = fill_prefill(fn, a, &k)) return rc;
+  if (int rc = check_workspace(fn, a->workspace, a->workspace_bytes, pl.total, 256)) return rc;
+  k.splits = pl.splits;
+  if (pl.splits > 1) {
+    k.part = (float*)a->workspace;
+    k.part_lse = (float*)((char*)a->workspace + pl.lse_off);
+  }
+  if (int rc = launch_rows(fn, stream, k, &a->params, pl.row_groups)) return rc;
+  if (pl.splits == 1) return FD_OK;
+  PrefillMergeArgs m;
+  memset(&m, 0, sizeof(m));
+  m.rows = k;
+  m.out_dtype = a->params.q_dtype;
+  const int rc = fd_launch_prefill_merge((hipStream_t)stream, m, a->params.head_dim);
+  if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
+  return FD_OK;
+}
+
+int64_t fd_decode_shared_workspace_bytes(const fd_shared_args* a) {
+  const char* fn = "fd_decode_shared_workspace_bytes";
+  if (!a) return fail(FD_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  if (a->step.batch == 0) return 0;
+  SharedPlan sp;
+  if (int rc = plan_shared(fn, a, &sp)) return rc;
+  return sp.total;
+}
+
+int fd_decode_shared(void* stream, const fd_shared_args* a) {
+  const char* fn = "fd_decode_shared";
+  if (!a) return fail(FD_ERR_INVALID_ARG, "%s: args is NULL", fn);
+  const fd_decode_args* st = &a->step;
+  if (st->batch == 0) return FD_OK;
+  SharedPlan sp;
+  if (int rc = plan_shared(fn, a, &sp)) return rc;
+  if (a->groups > 0 && (!a->prefix_table || !a->prefix_lens))
+    return fail(FD_ERR_INVALID_ARG, "%s: NULL prefix_table or prefix_lens", fn);
+  if (!st->kv_lens || !st->block_table) return fail(FD_ERR_INVALID_ARG, "%s: NULL tensor pointer", fn);
+  if (int rc = check_workspace(fn, st->workspace, st->workspace_bytes, sp.total, 256)) return rc;
+  char* ws = (char*)st->workspace;
+  const int D = st->params.head_dim;
+
+  // the prefixes: the sequences of a group are the rows of its tile, without a causal limit
+  fd_prefill_args pa;
+  memset(&pa, 0, sizeof(pa));
+  pa.q = st->q; pa.k = st->k_cache; pa.v = st->v_cache; pa.out = st->out; pa.lse_out = st->lse_out;
+  // (without groups the row-tile kernel is not launched; the pointers only have to pass the checks)
+  pa.cu_seqlens_q = a->group_starts;
+  pa.kv_lens = a->groups ? a->prefix_lens : st->kv_lens;
+  pa.block_table = a->groups ? a->prefix_table : st->block_table;
+  pa.stride_q_t = st->stride_q_bs; pa.stride_q_h = st->stride_q_h; pa.stride_k_tok = st->stride_k_tok;
+  pa.stride_k_h = st->stride_k_h; pa.stride_v_tok = st->stride_v_tok; pa.stride_v_h = st->stride_v_h;
+  pa.stride_ot = st->stride_obs; pa.stride_oh = st->stride_oh; pa.stride_table_bs = a->stride_prefix_bs;
+  pa.sm_scale = st->sm_scale; pa.batch = a->groups; pa.total_q = st->batch; pa.params = sp.prefix;
+  PrefillArgs k;
+  if (int rc = fill_prefill(fn, &pa, &k)) return rc;
+  k.splits = sp.rows.splits;
+  k.part = (float*)ws;
+  k.part_lse = (float*)(ws + sp.rows.lse_off);
+
+  // the sequences' own tokens
+  const int32_t* order = nullptr;
+  if (sp.step.order_kind != FD_ORDER_NONE) {
+    int32_t* o = (int32_t*)(ws + sp.order_off);
+    const int rc = sp.step.order_kind == FD_ORDER_ITEMS ? fd_schedule_items(stream, st->kv_lens, st->batch, o, &sp.step.p)
+                                                        : fd_schedule(stream, st->kv_lens, st->batch, o);
+    if (rc != FD_OK) return rc;
+    order = o;
+  }
+  if (a->groups > 0) {
+    if (int rc = launch_rows(fn, stream, k, &sp.prefix, sp.rows.row_groups)) return rc;
+  }
+  const int64_t S1 = sp.step.p.num_splits;
+  if (int rc = split_impl(fn, stream, st->q, st->k_cache, st->v_cache, ws + sp.own_off, (float*)(ws + sp.own_lse_off),
+                          st->sm_scale, st->block_table, st->kv_lens, st->batch, st->stride_q_bs, st->stride_q_h,
+                          st->stride_k_tok, st->stride_k_h, st->stride_v_tok, st->stride_v_h,
+                          (int64_t)st->params.q_heads * S1 * D, S1 * D, D, st->stride_table_bs, order, &sp.step.p, nullptr,
+                          nullptr))
+    return rc;
+  PrefillMergeArgs m;
+  memset(&m, 0, sizeof(m));
+  m.rows = k;
+  m.part1 = (const float*)(ws + sp.own_off);
+  m.part1_lse = (const float*)(ws + sp.own_lse_off);
+  m.S1 = (int)S1;
+  m.out_dtype = st->params.out_dtype;
+  const int rc = fd_launch_prefill_merge((hipStream_t)stream, m, D);
+  if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
+  return FD_OK;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Pages of a cache.
+
+namespace {
+
+int page_pool(const char* fn, const fd_page_pool* in, PagePool* out) {
+  if (!in) return fail(FD_ERR_INVALID_ARG, "%s: pool is NULL", fn);
+  if (!in->k_cache || !in->v_cache) return fail(FD_ERR_INVALID_ARG, "%s: NULL cache pointer", fn);
+  if (in->layers <= 0 || in->num_pages <= 0 || in->page_size <= 0)
+    return fail(FD_ERR_INVALID_ARG, "%s: layers %d, num_pages %d, page_size %d", fn, in->layers, in->num_pages,
+                in->page_size);
+  if (in->layers > 32767) return fail(FD_ERR_TOO_LARGE, "%s: %d layers (at most 32767)", fn, in->layers);
+  out->base[0] = (char*)in->k_cache; out->base[1] = (char*)in->v_cache;
+  out->layer_stride[0] = in->k_layer_stride; out->layer_stride[1] = in->v_layer_stride;
+  out->page_stride[0] = in->k_page_stride; out->page_stride[1] = in->v_page_stride;
+  out->page_bytes[0] = in->k_page_bytes; out->page_bytes[1] = in->v_page_bytes;
+  out->layers = in->layers; out->num_pages = in->num_pages; out->page_size = in->page_size;
+  for (int w = 0; w < 2; ++w) {
+    if (out->page_bytes[w] <= 0 || out->page_bytes[w] % ((int64_t)in->page_size * 16) || !aligned16(out->base[w]) ||
+        out->page_stride[w] % 16 || out->layer_stride[w] % 16)
+      return fail(FD_ERR_ALIGNMENT, "%s: pages must start on 16 bytes and hold a multiple of 16 bytes per token", fn);
+    if (out->page_stride[w] < out->page_bytes[w])
+      return fail(FD_ERR_INVALID_ARG, "%s: pages of %lld bytes, %lld apart", fn, (long long)out->page_bytes[w],
+                  (long long)out->page_stride[w]);
+  }
+  return FD_OK;
+}
+
+int page_tables(const char* fn, const fd_page_tables* in, PageTables* out, bool lens) {
+  if (!in) return fail(FD_ERR_INVALID_ARG, "%s: tables is NULL", fn);
+  if (!in->block_table || !in->page_refs || (lens && !in->kv_lens))
+    return fail(FD_ERR_INVALID_ARG, "%s: NULL table pointer", fn);
+  if (in->batch <= 0 || in->max_pages_per_seq <= 0 || in->stride_table_bs < 0)
+    return fail(FD_ERR_INVALID_ARG, "%s: batch %d, max_pages_per_seq %d", fn, in->batch, in->max_pages_per_seq);
+  out->bt = in->block_table; out->kv_lens = in->kv_lens; out->refs = in->page_refs; out->sbt = in->stride_table_bs;
+  out->batch = in->batch; out->width = in->max_pages_per_seq;
+  return FD_OK;
+}
+
+int page_result(const char* fn, int rc) {
+  if (rc == FD_ERR_TOO_LARGE) return fail(rc, "%s: batch or layers too large for one launch", fn);
+  if (rc != FD_OK) return fail(rc, "%s: launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
+  return FD_OK;
+}
+
+}  // namespace
+
+int64_t fd_pages_workspace_bytes(int32_t num_pages, int32_t count) {
+  if (num_pages < 0 || count < 0)
+    return fail(FD_ERR_INVALID_ARG, "fd_pages_workspace_bytes: num_pages %d, count %d", num_pages, count);
+  return count > 0 ? (int64_t)count * 12 : 16 + (int64_t)num_pages * 12;
+}
+
+int fd_pages_copy(void* stream, const fd_page_pool* pool, const int32_t* src_pages, const int32_t* dst_pages,
+                  int32_t count) {
+  const char* fn = "fd_pages_copy";
+  PagePool pp;
+  if (int rc = page_pool(fn, pool, &pp)) return rc;
+  if (count < 0) return fail(FD_ERR_INVALID_ARG, "%s: count %d", fn, count);
+  if (count == 0) return FD_OK;
+  if (!src_pages || !dst_pages) return fail(FD_ERR_INVALID_ARG, "%s: NULL page list", fn);
+  return page_result(fn, fd_launch_pages_copy((hipStream_t)stream, pp, src_pages, dst_pages, count));
+}
+
+int fd_pages_reserve(void* stream, const fd_page_tables* tables, int32_t num_pages, int32_t page_size,
+                     const int32_t* new_tokens, int32_t uniform, int32_t* ok) {
+  const char* fn = "fd_pages_reserve";
+  PageTables t;
+  if (int rc = page_tables(fn, tables, &t, true)) return rc;
+  if (num_pages <= 0 || page_size <= 0 || uniform < 0)
+    return fail(FD_ERR_INVALID_ARG, "%s: num_pages %d, page_size %d, new tokens %d", fn, num_pages, page_size, uniform);
+  if (!ok) return fail(FD_ERR_INVALID_ARG, "%s: ok is NULL", fn);
+  return page_result(fn, fd_launch_pages_reserve((hipStream_t)stream, t, num_pages, page_size, new_tokens, uniform, ok));
+}
+
+int fd_pages_fork(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, const int32_t* parents,
+                  const int32_t* children, int32_t count, int32_t* ok, void* workspace, int64_t workspace_bytes) {
+  const char* fn = "fd_pages_fork";
+  PagePool pp;
+  PageTables t;
+  if (int rc = page_pool(fn, pool, &pp)) return rc;
+  if (int rc = page_tables(fn, tables, &t, true)) return rc;
+  if (count < 0) return fail(FD_ERR_INVALID_ARG, "%s: count %d", fn, count);
+  if (count == 0) return FD_OK;
+  if (!parents || !children || !ok) return fail(FD_ERR_INVALID_ARG, "%s: NULL list", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, fd_pages_workspace_bytes(pp.num_pages, count), 16)) return rc;
+  return page_result(fn, fd_launch_pages_fork((hipStream_t)stream, pp, t, parents, children, count, ok, (int32_t*)workspace));
+}
+
+int fd_pages_free(void* stream, const fd_page_tables* tables, int32_t num_pages, const int32_t* rows, int32_t count) {
+  const char* fn = "fd_pages_free";
+  PageTables t;
+  if (int rc = page_tables(fn, tables, &t, true)) return rc;
+  if (num_pages <= 0 || count < 0) return fail(FD_ERR_INVALID_ARG, "%s: num_pages %d, count %d", fn, num_pages, count);
+  if (count == 0) return FD_OK;
+  if (!rows) return fail(FD_ERR_INVALID_ARG, "%s: rows is NULL", fn);
+  return page_result(fn, fd_launch_pages_free((hipStream_t)stream, t, num_pages, rows, count));
+}
+
+int fd_pages_compact(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, int32_t* live_out,
+                     void* workspace, int64_t workspace_bytes) {
+  const char* fn = "fd_pages_compact";
+  PagePool pp;
+  PageTables t;
+  if (int rc = page_pool(fn, pool, &pp)) return rc;
+  if (int rc = page_tables(fn, tables, &t, false)) return rc;
+  if (!live_out) return fail(FD_ERR_INVALID_ARG, "%s: live_out is NULL", fn);
+  if (int rc = check_workspace(fn, workspace, workspace_bytes, fd_pages_workspace_bytes(pp.num_pages, 0), 16)) return rc;
+  return page_result(fn, fd_launch_pages_compact((hipStream_t)stream, pp, t, live_out, (int32_t*)workspace));
+}
+
 }  // extern "C"

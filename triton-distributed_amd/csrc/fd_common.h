@@ -113,6 +113,53 @@ struct CombineArgs {
   int64_t s_lb, s_lh;
 };
 
+// Arguments of the prompt-attention kernel.
+struct PrefillArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;                // nullptr or [total_q, Hq]
+  float* part;               // nullptr (one split: out and lse), or fp32 partials [total_q, Hq, splits, D]
+  float* part_lse;           // ... and their LSEs [total_q, Hq, splits]
+  const int32_t* cu_q;       // [batch + 1], or nullptr: batch == 1, all rows
+  const int32_t* q_lens;     // nullptr, or [batch]: rows of a sequence behind its first q_lens are padding
+  const int32_t* cu_k;       // packed keys: [batch + 1]
+  const int32_t* kv_lens;    // paged keys: [batch]
+  const int32_t* bt;         // nullptr: packed keys
+  const float* k_scale;
+  const float* v_scale;
+  int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, so_t, so_h, sbt;
+  float sm_scale, soft_cap;
+  int32_t batch, total_q, total_k, Hq, Hkv, G, P, max_pages, num_pages, causal, splits;
+  uint32_t p_magic, p_shift;  // n / P
+  uint32_t g_magic, g_shift;  // n / G
+};
+
+// Arguments of the merge of two lists of partials per row (fd_prefill_merge.hip).
+struct PrefillMergeArgs {
+  PrefillArgs rows;          // rows, spans and outputs; part / part_lse / splits: the first list
+  const float* part1;        // nullptr, or the second list [total_q, Hq, S1, D] fp32, which every row has: rows outside the
+                             // spans are then merged from it alone instead of being left as they are
+  const float* part1_lse;    // [total_q, Hq, S1]
+  int32_t S1, out_dtype;
+};
+
+// A pair of page pools [layers, pages, P, heads, dim]; a page is contiguous, strides in bytes.
+struct PagePool {
+  char* base[2];             // K, V
+  int64_t layer_stride[2], page_stride[2], page_bytes[2];
+  int32_t layers, num_pages, page_size;
+};
+
+struct PageTables {
+  int32_t* bt;               // [batch, width]: pages of a row from the front, -1 behind them
+  int32_t* kv_lens;          // [batch]
+  int32_t* refs;             // [num_pages]: rows that hold a page, 0 = free
+  int64_t sbt;
+  int32_t batch, width;
+};
+
 // How a decode step cuts a sequence into ranges: what the scheduler needs to know of it.
 struct RangePlan {
   int32_t S;                  // ranges per sequence (grid slots)
@@ -1220,3 +1267,14 @@ int fd_launch_schedule(hipStream_t stream, const int32_t* kv_lens, int batch, in
 int fd_launch_schedule_items(hipStream_t stream, const int32_t* kv_lens, int batch, int64_t capacity,
                              const RangePlan& ranges, int32_t* items);
 int fd_launch_kv_append(hipStream_t stream, const AppendArgs& a, int src_dtype, int kv_dtype);
+int fd_launch_prefill_d64(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
+int fd_launch_prefill_d128(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
+int fd_launch_prefill_d256(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
+int fd_launch_prefill_merge(hipStream_t stream, const PrefillMergeArgs& a, int head_dim);
+int fd_launch_pages_copy(hipStream_t stream, const PagePool& pool, const int32_t* src, const int32_t* dst, int n);
+int fd_launch_pages_reserve(hipStream_t stream, const PageTables& t, int num_pages, int page_size,
+                            const int32_t* new_tokens, int uniform, int32_t* ok);
+int fd_launch_pages_fork(hipStream_t stream, const PagePool& pool, const PageTables& t, const int32_t* parents,
+                         const int32_t* children, int n, int32_t* ok, int32_t* ws);
+int fd_launch_pages_free(hipStream_t stream, const PageTables& t, int num_pages, const int32_t* rows, int n);
+int fd_launch_pages_compact(hipStream_t stream, const PagePool& pool, const PageTables& t, int32_t* live, int32_t* ws);

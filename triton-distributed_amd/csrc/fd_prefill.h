@@ -1,0 +1,505 @@
+// Attention of many query rows over packed keys or over the paged cache (gfx950): prompts, chunks of prompts, drafted
+// tokens, and the prefix part of a shared-prefix decode step.
+//
+// out[i,h] = sum_j softmax_j(scale q[i,h].k[j,h/G]) v[j,h/G] over the keys j that row i sees: j < n_k, and in the causal
+// form j <= i + n_k - n_q (the last query sees the last key).  One pass over the keys with the running maximum m and sum
+// l of the softmax; the accumulator is rescaled only when the maximum has grown by more than 2^8 (as in
+// fd_softmax_step).
+//
+// Rows: the G query heads of a KV head share its keys, so a row is a (token, head of the group) pair, r = token * G + head,
+// and a workgroup owns 32 * WR consecutive rows of one sequence and one KV head: a causal tile of G = 4 spans a quarter
+// of the tokens that 32 * WR rows of one head would, and wastes that much less on its diagonal.
+// Both products run on v_mfma_f32_32x32x16 with the scores transposed, S^T[token][row] = K Q^T and
+// O^T[dim][row] += V^T P^T: lane l then holds scores of row l % 32 only -- 16 of the 32 tokens of a block, tokens
+// 8 (i / 4) + 4 (l / 32) + i % 4 -- so a row's maximum and sum are in-lane reductions plus one exchange between the wave
+// halves, and those tokens are, eight at a time, exactly the k indices that the lane supplies as B operand of the second
+// product: P never leaves its registers.  V comes from LDS through the transposing read (ds_read_b64_tr_b16): 16 lanes
+// read four tokens of 16 dims and receive four tokens of one dim each.
+// Keys go global -> LDS without passing through registers (16-bit caches; 16 bytes a lane), two tiles deep.  The LDS image
+// of such a load is lane-linear, so rows are swizzled at the source: lane c of a row fetches the 16-byte chunk c ^ f(row),
+// with f chosen so that the 128-bit K reads (32 rows of one chunk column) and the transposing V reads (8 rows of 64 bytes)
+// both touch all 64 banks.  An fp8 cache is converted once per workgroup on its way to LDS (exact) instead.
+//
+// Tokens past a sequence's length are never fetched: the row address is clamped to the last token, and what such a row
+// holds is masked.  A masked score has weight 0, and 0 times a V row that is finite is 0; a V row that holds an infinity
+// or NaN would turn rows that do not see it into NaN, so a workgroup whose result is not finite runs once more with the
+// non-finite V values taken out of the masked tiles' products and added to the rows that see them only.
+#pragma once
+
+#include "fd_mma.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// The query rows of sequence b: `count` tokens from `start` on (whatever cu_q holds, inside [0, total_q)).  Without cu_q
+// there is one sequence, all rows.
+__device__ __forceinline__ void fd_prefill_span(const PrefillArgs& a, int b, int& start, int& count) {
+  start = 0;
+  count = a.total_q;
+  if (a.cu_q) {
+    start = min(max(a.cu_q[b], 0), a.total_q);
+    count = min(max(a.cu_q[b + 1], start), a.total_q) - start;
+  }
+  if (a.q_lens) count = min(count, max(a.q_lens[b], 0));
+}
+
+namespace {
+
+template <typename T>
+struct Mma32;
+template <>
+struct Mma32<__bf16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  }
+  static constexpr uint32_t kExp = 0x7f807f80u;   // exponent bits of both halves
+};
+template <>
+struct Mma32<_Float16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+  }
+  static constexpr uint32_t kExp = 0x7c007c00u;
+};
+
+// v and the other half's value of the same row
+__device__ __forceinline__ float half_max(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// 16 bytes per lane from global memory to lds_base + 16 * lane.  Inline assembly, so that the compiler does not put a wait
+// for it in front of the LDS reads of the other buffer; the kernel waits itself (vmcnt(0)) before the barrier that
+// publishes the tile.  The instruction has no register output.
+__device__ __forceinline__ void load_to_lds_b128(const void* src, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src)
+               : "memory", "m0");
+}
+
+__device__ __forceinline__ u32x4 lds_read_b128(const char* p) { return *(const u32x4*)p; }
+
+__device__ __forceinline__ u32x2 lds_read_tr(const char* p) {
+  typedef __attribute__((address_space(3))) i16x4* lds_ptr;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(i16x4*)p));
+}
+
+template <int D>
+struct PrefillTile {
+  static constexpr int kRowB = 2 * D;          // bytes of a 16-bit row in LDS
+  static constexpr int kChunks = D / 8;        // 16-byte chunks of it
+  // chunk c of row r lies at position c ^ k_swz(r) / c ^ v_swz(r) of the row
+  static __device__ __forceinline__ int k_swz(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int v_swz(int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; }
+};
+
+// T: query and product type.  FP8: e4m3 cache.  D: head dim.  WR row groups x WT token groups of waves, BN tokens a tile.
+template <typename T, bool FP8, int D, int WR, int WT, int BN>
+__global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_kernel(const PrefillArgs a) {
+  using Tile = PrefillTile<D>;
+  constexpr int NW = WR * WT;
+  constexpr int BM = 32 * WR;
+  constexpr int NT = BN / WT;              // tokens of a tile that a wave works on
+  constexpr int NB = NT / 32;              // ... in blocks of 32
+  constexpr int KS = D / 16;               // k steps of the scores
+  constexpr int MB = D / 32;               // dim blocks of the output
+  constexpr int kTileB = BN * Tile::kRowB; // bytes of a K (or V) tile in LDS
+  constexpr int kLoads = BN * Tile::kChunks / (64 * NW);     // 16-bit cache: loads per wave and operand
+  static_assert(NT % 32 == 0 && BN * Tile::kChunks % (64 * NW) == 0, "tile shape");
+  static_assert(4 * kTileB <= 65536, "two tiles of K and V within the reach of the direct loads' 16-bit LDS offset");
+  extern __shared__ __align__(1024) char smem[];             // [2][K tile, V tile]
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wr = wave % WR, wt = wave / WR;
+  const int half = lane >> 5, l32 = lane & 31;
+
+  // ---- work item: KV head fastest (the eight XCDs take neighbouring workgroups in turn, so with eight KV heads each
+  // XCD's L2 holds one head's keys), then the split, then the row tile
+  const int kvh = blockIdx.x % a.Hkv;
+  const int rest = blockIdx.x / a.Hkv;
+  const int split = rest % a.splits;
+  const int tile = rest / a.splits;
+  int b = -1, q_start = 0, n_q = 0, j = 0;
+  {
+    int base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 64) {
+      int s = 0, n = 0;
+      if (b0 + lane < a.batch) fd_prefill_span(a, b0 + lane, s, n);
+      const int tiles = (n * a.G + BM - 1) / BM;
+      int incl = tiles;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int up = __shfl_up(incl, off);
+        if (lane >= off) incl += up;
+      }
+      const uint64_t past = __ballot(base + incl > tile);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        b = b0 + at;
+        q_start = __builtin_amdgcn_readlane(s, at);
+        n_q = __builtin_amdgcn_readlane(n, at);
+        const int mine = __builtin_amdgcn_readlane(tiles, at);
+        // the tiles of a sequence from its end: in the causal form the ones with the most keys first
+        j = mine - 1 - (tile - base - (__builtin_amdgcn_readlane(incl, at) - mine));
+        break;
+      }
+      base += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  if (b < 0) return;
+
+  int n_k, k_start = 0;
+  if (a.bt) {
+    n_k = min(max(a.kv_lens[b], 0), a.max_pages * a.P);
+  } else {
+    k_start = min(max(a.cu_k[b], 0), a.total_k);
+    n_k = min(max(a.cu_k[b + 1], k_start), a.total_k) - k_start;
+  }
+  const int rows = n_q * a.G;
+  // keys that row r of the sequence sees: [0, limit)
+  auto token_of = [&](int r) { return (int)(((uint64_t)(uint32_t)r * a.g_magic) >> a.g_shift); };
+  auto limit_of = [&](int r) { return a.causal ? min(n_k, token_of(r) + 1 + n_k - n_q) : n_k; };
+  const int r0 = j * BM;
+  const int row = min(r0 + wr * 32 + l32, rows - 1);   // rows past the end repeat the last one and are not stored
+  const bool real_row = r0 + wr * 32 + l32 < rows;
+  const int q_tok = token_of(row), q_head = row - q_tok * a.G;
+  const int my_limit = limit_of(row);
+  const int wave_lo = limit_of(min(r0 + wr * 32, rows - 1));            // the wave's rows see at least this many keys
+  const int wave_hi = limit_of(min(r0 + wr * 32 + 31, rows - 1));       // ... and at most this many
+  const int wg_hi = limit_of(min(r0 + BM - 1, rows - 1));
+  const int all_tiles = (max(wg_hi, 0) + BN - 1) / BN;
+  const int per_split = (all_tiles + a.splits - 1) / a.splits;
+  const int t_first = min(split * per_split, all_tiles);
+  const int t_last = min(t_first + per_split, all_tiles);
+
+  // ---- Q^T as B operand: lane (row, half) holds dims 16 ks + 8 half .. + 7
+  u32x4 qf[KS];
+  {
+    const char* qp = (const char*)a.q + 2 * ((int64_t)(q_start + q_tok) * a.sq_t + (int64_t)(kvh * a.G + q_head) * a.sq_h);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = *(const u32x4*)(qp + 32 * ks + 16 * half);
+  }
+  float c = a.sm_scale;
+  if (FP8) c *= a.k_scale[kvh];
+  float cap = 0.f, cap_in = 0.f;
+  if (a.soft_cap > 0.f) {         // x = cap tanh(s c / cap), in the base-2 domain afterwards
+    cap_in = c / a.soft_cap;
+    cap = a.soft_cap * FD_LOG2E;
+    c = 1.f;
+  } else {
+    // the maximum is taken over the raw scores, so the factor has to be positive: a negative one goes into Q (exact)
+    if (c < 0.f) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qf[ks] ^= 0x80008000u;
+    }
+    c = fmaxf(fabsf(c) * FD_LOG2E, 1e-30f);
+  }
+
+  // ---- addresses
+  const int ksw = Tile::k_swz(l32);                     // row of a K read: l32 + a multiple of 32
+  const int k_lane = (wt * NT + l32) * Tile::kRowB + ((half ^ ksw) << 4);
+  const int vi = lane & 15;
+  const int v_tok = wt * NT + 4 * half + (vi >> 2);
+  const int v_lane = v_tok * Tile::kRowB + ((lane >> 4) & 1) * 32 + (vi & 3) * 8;
+  const int v_swz = Tile::v_swz(v_tok) << 4;            // the same for all token steps of 8
+  const char* kb = (const char*)a.k + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sk_h);
+  const char* vb = (const char*)a.v + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sv_h);
+  const int64_t sk_b = a.sk_t * (FP8 ? 1 : 2), sv_b = a.sv_t * (FP8 ? 1 : 2);
+  const int32_t* table = a.bt ? a.bt + (int64_t)b * a.sbt : nullptr;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+
+  // The token row in the pool of token t0 + lane of a tile (lanes past BN repeat the last): page entry first, so that it
+  // can be requested a tile early.
+  auto page_entry = [&](int t) -> int {
+    if (!table) return 0;
+    const int tok = min(t * BN + min(lane, BN - 1), n_k - 1);
+    const int pg = (int)(((uint64_t)(uint32_t)tok * a.p_magic) >> a.p_shift);
+    return table[pg];
+  };
+  auto pool_row = [&](int t, int entry) -> int {
+    const int tok = min(t * BN + min(lane, BN - 1), n_k - 1);
+    if (!table) return k_start + tok;
+    const int pg = (int)(((uint64_t)(uint32_t)tok * a.p_magic) >> a.p_shift);
+    return min(max(entry, 0), a.num_pages - 1) * a.P + (tok - pg * a.P);
+  };
+
+  // ---- tile loads.  16-bit: chunk n = (i NW + wave) 64 + lane of the tile's LDS image.  fp8: through registers.
+  constexpr int kF8Loads = FP8 ? BN * D / 16 / (64 * NW) : 1;
+  u32x4 f8k[kF8Loads], f8v[kF8Loads];
+  auto request = [&](int buf, int rows_of_tile) {
+    if constexpr (!FP8) {
+      const uint32_t at = lds0 + buf * 2 * kTileB;
+#pragma unroll (kLoads > 8 ? 4 : kLoads)   // (more addresses at once than the registers beside a 256-wide head hold)
+      for (int i = 0; i < kLoads; ++i) {
+        const int n = (i * NW + wave) * 64 + lane;
+        const int r = n / Tile::kChunks, ch = n % Tile::kChunks;
+        const int64_t pr = __shfl(rows_of_tile, r);
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(at + (i * NW + wave) * 1024);
+        load_to_lds_b128(kb + pr * sk_b + ((ch ^ Tile::k_swz(r)) << 4), dst);
+        load_to_lds_b128(vb + pr * sv_b + ((ch ^ Tile::v_swz(r)) << 4), dst + kTileB);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kF8Loads; ++i) {
+        const int n = (i * NW + wave) * 64 + lane;
+        const int r = n / (D / 16), ch = n % (D / 16);
+        const int64_t pr = __shfl(rows_of_tile, r);
+        f8k[i] = *(const u32x4*)(kb + pr * sk_b + (ch << 4));
+        f8v[i] = *(const u32x4*)(vb + pr * sv_b + (ch << 4));
+      }
+    }
+  };
+  auto deposit = [&](int buf) {   // fp8: convert what `request` fetched and put it into LDS
+    if constexpr (FP8) {
+      char* at = smem + buf * 2 * kTileB;
+#pragma unroll
+      for (int i = 0; i < kF8Loads; ++i) {
+        const int n = (i * NW + wave) * 64 + lane;
+        const int r = n / (D / 16), ch = n % (D / 16);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          u32x4 k16, v16;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            k16[2 * w] = Mma<T>::from_fp8(f8k[i][2 * h + w], false);
+            k16[2 * w + 1] = Mma<T>::from_fp8(f8k[i][2 * h + w], true);
+            v16[2 * w] = Mma<T>::from_fp8(f8v[i][2 * h + w], false);
+            v16[2 * w + 1] = Mma<T>::from_fp8(f8v[i][2 * h + w], true);
+          }
+          *(u32x4*)(at + r * Tile::kRowB + (((2 * ch + h) ^ Tile::k_swz(r)) << 4)) = k16;
+          *(u32x4*)(at + kTileB + r * Tile::kRowB + (((2 * ch + h) ^ Tile::v_swz(r)) << 4)) = v16;
+        }
+      }
+    }
+  };
+
+  f32x16 o[MB];
+  float m, l;
+  bool careful = false;
+  for (;;) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) o[mb] = f32x16{};
+    m = -3.0e38f;     // below every score: a row that sees nothing keeps l = 0
+    l = 0.f;
+    int entry = 0;
+    if (t_first < t_last) {
+      const int rows0 = pool_row(t_first, page_entry(t_first));
+      request(0, rows0);
+      if (t_first + 1 < t_last) entry = page_entry(t_first + 1);
+      deposit(0);
+    }
+    for (int t = t_first; t < t_last; ++t) {
+      const int buf = (t - t_first) & 1;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();      // tile t is in LDS, and nobody reads the other buffer any more
+      if (t + 1 < t_last) {
+        const int next = pool_row(t + 1, entry);
+        if (t + 2 < t_last) entry = page_entry(t + 2);
+        request(buf ^ 1, next);
+      }
+      const int t0 = t * BN + wt * NT;       // first token of this wave's part
+      if (t0 < wave_hi) {
+        const char* kt = smem + buf * 2 * kTileB;
+        const char* vt = smem + buf * 2 * kTileB + kTileB + v_lane;
+        f32x16 s[NB];
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) {
+          s[tb] = f32x16{};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const u32x4 kf = lds_read_b128(kt + (k_lane ^ (ks << 5)) + tb * 32 * Tile::kRowB);
+            s[tb] = Mma32<T>::run(kf, qf[ks], s[tb]);
+          }
+        }
+        if (a.soft_cap > 0.f) {
+#pragma unroll
+          for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float e = fd_exp2(2.0f * FD_LOG2E * s[tb][i] * cap_in);
+              s[tb][i] = cap * (1.0f - 2.0f / (1.0f + e));
+            }
+        }
+        const bool masked = t0 + NT > wave_lo;
+        if (masked) {
+          const int see = my_limit - t0 - 4 * half;
+#pragma unroll
+          for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              s[tb][i] = tb * 32 + 8 * (i / 4) + i % 4 < see ? s[tb][i] : -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
+        mx = half_max(mx) * c;
+        const float top = fmaxf(m, mx);
+        const float m_new = top - m > 8.0f ? top : m;
+        if (__any(m_new > m)) {
+          const float alpha = fd_exp2(m - m_new);
+          l *= alpha;
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) o[mb] *= alpha;
+          m = m_new;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[tb][i] = fd_exp2(__builtin_fmaf(s[tb][i], c, -m));
+            sum += s[tb][i];
+          }
+        l += sum;
+        // P is rounded to the query's type for the second product (the sum l is not): half a step, 2^-9 (bf16) or 2^-12
+        // (fp16) of each weight, below the rounding of the output itself
+#pragma unroll
+        for (int st = 0; st < NT / 16; ++st) {
+          u32x4 pf;
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            pf[w] = Mma<T>::pack(s[st / 2][8 * (st % 2) + 2 * w], s[st / 2][8 * (st % 2) + 2 * w + 1]);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            const char* vp = vt + st * 16 * Tile::kRowB + ((mb << 6) ^ v_swz);
+            const u32x2 lo = lds_read_tr(vp), hi = lds_read_tr(vp + 8 * Tile::kRowB);
+            u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+            if (careful && masked) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) {
+                const uint32_t e = vf[w] & Mma32<T>::kExp;
+                if ((e & 0xffffu) == (Mma32<T>::kExp & 0xffffu)) vf[w] &= 0xffff0000u;
+                if ((e >> 16) == (Mma32<T>::kExp >> 16)) vf[w] &= 0xffffu;
+              }
+            }
+            o[mb] = Mma32<T>::run(vf, pf, o[mb]);
+          }
+        }
+        if (careful && masked) {
+          // the non-finite V values of this tile, for the rows that see them: lane (row, half) owns dims
+          // 32 mb + 8 i + 4 half .. + 3
+          for (int n = 0; n < NT; ++n) {
+            if (t0 + n >= my_limit) continue;
+            const int r = wt * NT + n;
+            const char* vr = smem + buf * 2 * kTileB + kTileB + r * Tile::kRowB;
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int d0 = 32 * mb + 8 * i + 4 * half;
+                const u32x2 w = *(const u32x2*)(vr + ((((d0 >> 3) ^ Tile::v_swz(r)) << 4) | ((d0 & 4) << 1)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint16_t bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                  if ((bits & (uint16_t)Mma32<T>::kExp) == (uint16_t)Mma32<T>::kExp)
+                    o[mb][4 * i + e] += (float)__builtin_bit_cast(T, bits);
+                }
+              }
+          }
+        }
+      }
+      if (t + 1 < t_last) deposit(buf ^ 1);
+    }
+    if (careful || t_first == t_last) break;
+    // any value that is not finite?  (x - x is 0 for finite x)
+    float probe = l - l;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) probe += o[mb][i] - o[mb][i];
+    volatile int* flag = (volatile int*)smem;   // the tiles are used up
+    __syncthreads();
+    if (threadIdx.x == 0) *flag = 0;
+    __syncthreads();
+    if (__any(!(probe == 0.f)) && lane == 0) *flag = 1;
+    __syncthreads();
+    const bool again = *flag != 0;
+    __syncthreads();
+    if (!again) break;
+    careful = true;
+  }
+
+  // ---- join the token groups, store
+  l = half_sum(l);
+  if constexpr (WT > 1) {
+    static_assert(WT == 2, "two token groups");
+    static_assert(WR * (D * 32 + 64) * 4 <= 4 * kTileB, "the second group's state fits over the tiles");
+    float* st = (float*)smem + wr * (D * 32 + 64);
+    __syncthreads();
+    if (wt == 1) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[(mb * 16 + i) * 64 + lane] = o[mb][i];
+      if (half == 0) {
+        st[D * 32 + l32] = m;
+        st[D * 32 + 32 + l32] = l;
+      }
+    }
+    __syncthreads();
+    if (wt == 1) return;
+    const float m1 = st[D * 32 + l32], l1 = st[D * 32 + 32 + l32];
+    const float top = fmaxf(m, m1);
+    const float f0 = fd_exp2(m - top), f1 = fd_exp2(m1 - top);
+    l = l * f0 + l1 * f1;
+    m = top;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[mb][i] = o[mb][i] * f0 + st[(mb * 16 + i) * 64 + lane] * f1;
+  }
+  if (!real_row) return;
+  float inv = l != 0.f ? 1.0f / l : 0.f;
+  const float lse = l != 0.f ? m * FD_LN2 + __logf(l) : -INFINITY;
+  if (FP8) inv *= a.v_scale[kvh];
+  const int64_t tok = q_start + q_tok;
+  const int head = kvh * a.G + q_head;
+  if (a.part) {
+    const int64_t pr = (tok * a.Hq + head) * a.splits + split;
+    if (half == 0) a.part_lse[pr] = lse;
+    if (l == 0.f) return;         // weight 0: the row is not looked at
+    float* dst = a.part + pr * D;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *(f32x4*)(dst + 32 * mb + 8 * i + 4 * half) =
+            f32x4{o[mb][4 * i] * inv, o[mb][4 * i + 1] * inv, o[mb][4 * i + 2] * inv, o[mb][4 * i + 3] * inv};
+  } else {
+    if (a.lse && half == 0) a.lse[tok * a.Hq + head] = lse;
+    char* dst = (char*)a.out + 2 * (tok * a.so_t + (int64_t)head * a.so_h);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x2 w = {Mma<T>::pack(o[mb][4 * i] * inv, o[mb][4 * i + 1] * inv),
+                   Mma<T>::pack(o[mb][4 * i + 2] * inv, o[mb][4 * i + 3] * inv)};
+        *(u32x2*)(dst + 2 * (32 * mb + 8 * i + 4 * half)) = w;
+      }
+  }
+}
+
+template <typename T, bool FP8, int D, int WR, int WT, int BN>
+int launch_prefill(hipStream_t stream, const PrefillArgs& a) {
+  constexpr int BM = 32 * WR;
+  constexpr size_t lds = 4 * BN * 2 * D;
+  const int64_t tiles = ((int64_t)a.total_q * a.G + (int64_t)a.batch * (BM - 1)) / BM;   // sum of ceil(rows_b / BM) at most
+  const int64_t wgs = tiles * a.splits * a.Hkv;
+  if (wgs >= ((int64_t)1 << 31)) return FD_ERR_TOO_LARGE;
+  if (wgs == 0) return FD_OK;
+  auto kern = fd_prefill_kernel<T, FP8, D, WR, WT, BN>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * WR * WT), lds, stream, a);
+  return hipGetLastError() == hipSuccess ? FD_OK : FD_ERR_LAUNCH;
+}
+
+}  // namespace

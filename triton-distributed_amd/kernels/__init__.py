@@ -24,8 +24,28 @@ from .kv_append import (  # noqa: F401
     paged_kv_append,
     rope_kv_append,
 )
+from .pages import (  # noqa: F401
+    paged_kv_compact,
+    paged_kv_copy,
+    paged_kv_fork,
+    paged_kv_free,
+    paged_kv_reserve,
+)
+from .prefill import (  # noqa: F401
+    gqa_fwd_batch_decode_shared_prefix,
+    gqa_fwd_batch_prefill,
+    prefill_workspace_bytes,
+)
 
 __all__ = [
+    "gqa_fwd_batch_prefill",
+    "gqa_fwd_batch_decode_shared_prefix",
+    "prefill_workspace_bytes",
+    "paged_kv_copy",
+    "paged_kv_reserve",
+    "paged_kv_fork",
+    "paged_kv_free",
+    "paged_kv_compact",
     "apply_rotary_pos_emb",
     "flash_attn_with_kvcache",
     "paged_kv_append",

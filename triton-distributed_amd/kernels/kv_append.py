@@ -23,6 +23,7 @@ from .._lib import FdParams, FdQkPrep, check, fd_dtype_of, load_library, stream_
 from .._lib import (FD_ORDER_ITEMS, FD_ORDER_SEQUENCES, FD_STEP_EXACT_SPLITS, FD_STEP_FUSED,
                     FD_STEP_ORDER_FROM_APPEND)
 from .flash_decode import _decode, _require_cuda, decode_plan, item_order_buffer
+from .prefill import gqa_fwd_batch_decode_shared_prefix
 
 
 def _ptr(t: Optional[torch.Tensor]):
@@ -179,7 +180,7 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
                             window_size=(-1, -1), softcap=0.0, rotary_interleaved=True, alibi_slopes=None,
                             num_splits=0, return_softmax_lse=False, *, cos_sin_cache=None, position_ids=None,
                             k_scale=None, v_scale=None, kv_lens_out=None, q_norm=None, k_norm=None, stream=None,
-                            **decode_kw):
+                            shared_prefix=None, **decode_kw):
     """Decode-step drop-in for the flash-attn call of the reference's attention block (tp_attn.py:268-269).
 
     ``q [B, 1, Hq, D]``; ``k_cache`` / ``v_cache`` either dense ``[B_cache, L, Hkv, D]`` (the reference's
@@ -193,7 +194,10 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     on the way in, in the append launch, after the per-head RMS norms ``q_norm`` / ``k_norm`` =
     ``(weight, eps)``; ``k_scale`` / ``v_scale`` select an fp8-e4m3 cache;
     ``kv_lens_out`` receives ``cache_seqlens + T``.  ``num_splits`` 0 lets the library choose.
-    Not covered, and refused: more than one query token, flash-attn's own rotary arguments, left padding,
+    ``shared_prefix`` = ``(prefix_lens, prefix_table, group_starts or None)``: sequences that share prefixes
+    (``gqa_fwd_batch_decode_shared_prefix``); ``block_table`` and ``cache_seqlens`` then describe what each
+    sequence holds behind its group's prefix.
+    Not covered, and refused: more than one query token (``gqa_fwd_batch_prefill``), flash-attn's own rotary arguments, left padding,
     sliding windows and ALiBi.
     """
     if q.dim() != 4 or q.shape[1] != 1:
@@ -226,7 +230,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         if kv_lens_out is None:
             kv_lens_out = torch.empty_like(cache_seqlens)
         order = items = item_plan = None
-        if "seq_order" not in decode_kw and "item_order" not in decode_kw and decode_kw.get("auto_order", True):
+        if (shared_prefix is None and "seq_order" not in decode_kw and "item_order" not in decode_kw
+                and decode_kw.get("auto_order", True)):
             # the append launch can also compute the decode's issue order, at no launch of its own: the library's
             # plan says whether that pays for this batch and which kind -- (sequence, range) items, largest first, or
             # sequences, longest first
@@ -259,6 +264,13 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
 
     out = torch.empty_like(q)
     lse = torch.empty((bsz, q_heads), dtype=torch.float32, device=dev) if return_softmax_lse else None
+    if shared_prefix is not None:
+        prefix_lens, prefix_table, group_starts = shared_prefix
+        gqa_fwd_batch_decode_shared_prefix(q_rot[:, 0], k_cache, v_cache, None, None, kv_lens, block_table, prefix_lens,
+                                           prefix_table, scale, softcap, group_starts=group_starts,
+                                           output_combine=out[:, 0], lse_out=lse, k_scale=k_scale, v_scale=v_scale,
+                                           stream=stream, **decode_kw)
+        return (out, lse.view(bsz, q_heads, 1)) if return_softmax_lse else out
     _decode(q_rot.view(bsz, q_heads, head_dim) if q_rot.is_contiguous() else q_rot[:, 0], k_cache, v_cache, None,
             kv_lens, block_table, scale, softcap, None, out.view(bsz, q_heads, head_dim),
             num_splits if num_splits > 0 else -1, with_lse_column=False, lse_out=lse, k_scale=k_scale, v_scale=v_scale,

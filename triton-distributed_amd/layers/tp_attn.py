@@ -8,16 +8,19 @@ the split-KV decode of this package instead of the flash-attn package (tp_attn.p
 projections stay plain ``torch.nn.functional.linear`` calls (hipBLASLt), as in the reference's
 ``torch_fwd``.
 
-Only the decode step (one new token per sequence) on one GPU is covered: ``world_size`` must be 1 -- the
-all-gather / reduce-scatter GEMMs of ``dist_triton_fwd`` (tp_attn.py:278-306) and the prefill attention are
-other paths -- and anything else raises.
+``fwd`` is the decode step (one new token per sequence), ``prefill`` the same block for prompts and chunks of them.
+One GPU: ``world_size`` must be 1 -- the all-gather / reduce-scatter GEMMs of ``dist_triton_fwd`` (tp_attn.py:278-306)
+are other paths -- and anything else raises.
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 from torch import nn
 
-from ..kernels.kv_append import flash_attn_with_kvcache
+from ..kernels.kv_append import _dense_block_table, flash_attn_with_kvcache, rope_kv_append
+from ..kernels.prefill import gqa_fwd_batch_prefill
 
 
 def layer_norm(hidden_states: torch.Tensor, eps: float, w: torch.Tensor):
@@ -98,6 +101,41 @@ class TP_Attn:
                                       block_table=kv_cache.block_table, causal=True, cos_sin_cache=cos_sin_cache,
                                       position_ids=position_ids, k_scale=kv_cache.k_scale, v_scale=kv_cache.v_scale,
                                       q_norm=q_norm, k_norm=k_norm, **decode_kw)
+        return nn.functional.linear(out.view(bsz, q_len, -1), self.wo)
+
+    @torch.inference_mode()
+    def prefill(self, x: torch.Tensor, position_ids: torch.Tensor, cos_sin_cache: torch.Tensor, kv_cache, layer_idx: int,
+                q_lens: Optional[torch.Tensor] = None, **prefill_kw):
+        """x ``[B, T, hidden]`` -> ``[B, T, hidden]``: T new tokens per sequence behind what ``kv_cache`` holds at its
+        offsets -- a whole prompt, or the next chunk of one.  Their K/V are appended in one launch (norms, rotary and fp8
+        included), then causal attention covers cache and chunk.  ``q_lens`` (int32 ``[B]``): a batch padded to T, only the
+        first ``q_lens[b]`` tokens of sequence b are real; what the padding wrote behind a sequence's length is
+        overwritten by its next tokens, and its rows of the result mean nothing.  The caller advances the offsets
+        (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  Keywords go to ``gqa_fwd_batch_prefill``."""
+        bsz, q_len, _ = x.size()
+        if q_len == 0:
+            return x.new_empty(bsz, 0, self.wo.shape[0])
+        qkv = nn.functional.linear(x, self.wqkv)
+        q, k, v = (t.view(bsz, q_len, -1, self.head_dim)
+                   for t in qkv.split([self.q_size, self.kv_size, self.kv_size], dim=-1))
+        q_norm = (self.q_norm_w, self.q_norm_eps) if hasattr(self, "q_norm_eps") else None
+        k_norm = (self.k_norm_w, self.k_norm_eps) if hasattr(self, "k_norm_eps") else None
+        k_cache, v_cache, kv_offset = kv_cache.update_kv_cache(k, v, layer_idx)
+        table = kv_cache.block_table if kv_cache.block_table is not None else _dense_block_table(x.device, bsz)
+        kv_lens = torch.empty_like(kv_offset)
+        prep_q = cos_sin_cache is not None or q_norm is not None
+        q_rows = torch.empty(q.shape, dtype=q.dtype, device=q.device) if prep_q else q
+        rope_kv_append(k, v, k_cache, v_cache, table, kv_offset, kv_lens_out=kv_lens, k_scale=kv_cache.k_scale,
+                       v_scale=kv_cache.v_scale, cos_sin=cos_sin_cache, position_ids=position_ids,
+                       q=q if prep_q else None, q_out=q_rows if prep_q else None, q_norm=q_norm, k_norm=k_norm)
+        out = None
+        if q_lens is not None:
+            kv_lens = torch.minimum(kv_offset + q_lens, kv_lens)
+            out = torch.zeros(bsz * q_len, q.shape[2], self.head_dim, dtype=q.dtype, device=q.device)
+        starts = torch.arange(0, bsz * q_len + 1, q_len, dtype=torch.int32, device=x.device)
+        out = gqa_fwd_batch_prefill(q_rows.reshape(bsz * q_len, -1, self.head_dim), k_cache, v_cache, starts, kv_lens, table,
+                                    self.head_dim ** -0.5, q_lens=q_lens, output=out, k_scale=kv_cache.k_scale,
+                                    v_scale=kv_cache.v_scale, **prefill_kw)
         return nn.functional.linear(out.view(bsz, q_len, -1), self.wo)
 
     torch_fwd = fwd

@@ -100,8 +100,8 @@ struct PrefillTile {
   static __device__ __forceinline__ int v_swz(int r) { return D == 64 ? ((r >> 1) & 1) << 2 : (r & 3) << 2; }
 };
 
-// T: query and product type.  FP8: e4m3 cache.  D: head dim.  WR row groups x WT token groups of waves, BN tokens a tile.
-template <typename T, bool FP8, int D, int WR, int WT, int BN>
+// T: query and product type.  FP8: e4m3 cache.  CAP: soft-capped scores.  D: head dim.  WR row groups x WT token groups of waves, BN tokens a tile.
+template <typename T, bool FP8, bool CAP, int D, int WR, int WT, int BN>
 __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_kernel(const PrefillArgs a) {
   using Tile = PrefillTile<D>;
   constexpr int NW = WR * WT;
@@ -111,7 +111,6 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   constexpr int KS = D / 16;               // k steps of the scores
   constexpr int MB = D / 32;               // dim blocks of the output
   constexpr int kTileB = BN * Tile::kRowB; // bytes of a K (or V) tile in LDS
-  constexpr int kLoads = BN * Tile::kChunks / (64 * NW);     // 16-bit cache: loads per wave and operand
   static_assert(NT % 32 == 0 && BN * Tile::kChunks % (64 * NW) == 0, "tile shape");
   static_assert(4 * kTileB <= 65536, "two tiles of K and V within the reach of the direct loads' 16-bit LDS offset");
   extern __shared__ __align__(1024) char smem[];             // [2][K tile, V tile]
@@ -173,7 +172,6 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const int q_tok = token_of(row), q_head = row - q_tok * a.G;
   const int my_limit = limit_of(row);
   const int wave_lo = limit_of(min(r0 + wr * 32, rows - 1));            // the wave's rows see at least this many keys
-  const int wave_hi = limit_of(min(r0 + wr * 32 + 31, rows - 1));       // ... and at most this many
   const int wg_hi = limit_of(min(r0 + BM - 1, rows - 1));
   const int all_tiles = (max(wg_hi, 0) + BN - 1) / BN;
   const int per_split = (all_tiles + a.splits - 1) / a.splits;
@@ -190,8 +188,8 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   float c = a.sm_scale;
   if (FP8) c *= a.k_scale[kvh];
   float cap = 0.f, cap_in = 0.f;
-  if (a.soft_cap > 0.f) {         // x = cap tanh(s c / cap), in the base-2 domain afterwards
-    cap_in = c / a.soft_cap;
+  if constexpr (CAP) {            // x = cap tanh(s c / cap), in the base-2 domain afterwards
+    cap_in = 2.0f * FD_LOG2E * c / a.soft_cap;
     cap = a.soft_cap * FD_LOG2E;
     c = 1.f;
   } else {
@@ -212,7 +210,7 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const int v_swz = Tile::v_swz(v_tok) << 4;            // the same for all token steps of 8
   const char* kb = (const char*)a.k + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sk_h);
   const char* vb = (const char*)a.v + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sv_h);
-  const int64_t sk_b = a.sk_t * (FP8 ? 1 : 2), sv_b = a.sv_t * (FP8 ? 1 : 2);
+  const uint32_t sk_b = (uint32_t)a.sk_t * (FP8 ? 1 : 2), sv_b = (uint32_t)a.sv_t * (FP8 ? 1 : 2);
   const int32_t* table = a.bt ? a.bt + (int64_t)b * a.sbt : nullptr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
 
@@ -232,185 +230,294 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   };
 
   // ---- tile loads.  16-bit: chunk n = (i NW + wave) 64 + lane of the tile's LDS image.  fp8: through registers.
-  constexpr int kF8Loads = FP8 ? BN * D / 16 / (64 * NW) : 1;
-  u32x4 f8k[kF8Loads], f8v[kF8Loads];
-  auto request = [&](int buf, int rows_of_tile) {
-    if constexpr (!FP8) {
-      const uint32_t at = lds0 + buf * 2 * kTileB;
-#pragma unroll (kLoads > 8 ? 4 : kLoads)   // (more addresses at once than the registers beside a 256-wide head hold)
-      for (int i = 0; i < kLoads; ++i) {
-        const int n = (i * NW + wave) * 64 + lane;
-        const int r = n / Tile::kChunks, ch = n % Tile::kChunks;
-        const int64_t pr = __shfl(rows_of_tile, r);
-        const uint32_t dst = __builtin_amdgcn_readfirstlane(at + (i * NW + wave) * 1024);
-        load_to_lds_b128(kb + pr * sk_b + ((ch ^ Tile::k_swz(r)) << 4), dst);
-        load_to_lds_b128(vb + pr * sv_b + ((ch ^ Tile::v_swz(r)) << 4), dst + kTileB);
-      }
-    } else {
+  constexpr int kChunksLoaded = FP8 ? D / 16 : Tile::kChunks;         // 16-byte chunks of a row in memory
+  constexpr int kLoads = BN * kChunksLoaded / (64 * NW);              // loads per lane and operand
+  int pr[kLoads];                                                     // pool rows that this lane fetches from
+  u32x4 f8k[FP8 ? kLoads : 1], f8v[FP8 ? kLoads : 1];
+  auto rows_of = [&](int rows_of_tile) {
 #pragma unroll
-      for (int i = 0; i < kF8Loads; ++i) {
-        const int n = (i * NW + wave) * 64 + lane;
-        const int r = n / (D / 16), ch = n % (D / 16);
-        const int64_t pr = __shfl(rows_of_tile, r);
-        f8k[i] = *(const u32x4*)(kb + pr * sk_b + (ch << 4));
-        f8v[i] = *(const u32x4*)(vb + pr * sv_b + (ch << 4));
+    for (int i = 0; i < kLoads; ++i) pr[i] = __shfl(rows_of_tile, ((i * NW + wave) * 64 + lane) / kChunksLoaded);
+  };
+  // (a pool has fewer than 2^31 rows and a row stride fits 32 bits: one 32 x 32 -> 64 bit multiply)
+  auto request = [&](bool is_k, int buf) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int n = (i * NW + wave) * 64 + lane;
+      const int r = n / kChunksLoaded, ch = n % kChunksLoaded;
+      const char* src = (is_k ? kb : vb) + (uint64_t)(uint32_t)pr[i] * (is_k ? sk_b : sv_b);
+      if constexpr (FP8) {
+        (is_k ? f8k : f8v)[i] = *(const u32x4*)(src + (ch << 4));
+      } else {
+        const uint32_t dst = lds0 + (2 * buf + (is_k ? 0 : 1)) * kTileB + (i * NW + wave) * 1024;
+        load_to_lds_b128(src + ((ch ^ (is_k ? Tile::k_swz(r) : Tile::v_swz(r))) << 4), __builtin_amdgcn_readfirstlane(dst));
       }
     }
   };
-  auto deposit = [&](int buf) {   // fp8: convert what `request` fetched and put it into LDS
+  auto deposit = [&](bool is_k, int buf) {   // fp8: convert what `request` fetched and put it into LDS
     if constexpr (FP8) {
-      char* at = smem + buf * 2 * kTileB;
+      char* at = smem + (2 * buf + (is_k ? 0 : 1)) * kTileB;
 #pragma unroll
-      for (int i = 0; i < kF8Loads; ++i) {
+      for (int i = 0; i < kLoads; ++i) {
         const int n = (i * NW + wave) * 64 + lane;
-        const int r = n / (D / 16), ch = n % (D / 16);
+        const int r = n / kChunksLoaded, ch = n % kChunksLoaded;
+        const u32x4 raw = (is_k ? f8k : f8v)[i];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          u32x4 k16, v16;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            k16[2 * w] = Mma<T>::from_fp8(f8k[i][2 * h + w], false);
-            k16[2 * w + 1] = Mma<T>::from_fp8(f8k[i][2 * h + w], true);
-            v16[2 * w] = Mma<T>::from_fp8(f8v[i][2 * h + w], false);
-            v16[2 * w + 1] = Mma<T>::from_fp8(f8v[i][2 * h + w], true);
-          }
-          *(u32x4*)(at + r * Tile::kRowB + (((2 * ch + h) ^ Tile::k_swz(r)) << 4)) = k16;
-          *(u32x4*)(at + kTileB + r * Tile::kRowB + (((2 * ch + h) ^ Tile::v_swz(r)) << 4)) = v16;
+          const u32x4 x = {Mma<T>::from_fp8(raw[2 * h], false), Mma<T>::from_fp8(raw[2 * h], true),
+                           Mma<T>::from_fp8(raw[2 * h + 1], false), Mma<T>::from_fp8(raw[2 * h + 1], true)};
+          *(u32x4*)(at + r * Tile::kRowB + (((2 * ch + h) ^ (is_k ? Tile::k_swz(r) : Tile::v_swz(r))) << 4)) = x;
         }
       }
+    }
+  };
+  auto publish = [&] {   // what was requested is in LDS, for every wave, and nobody reads what is requested next
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+
+  // ---- the pieces of a tile's work
+  auto k_frag = [&](int buf, int ks, int tb) {
+    return lds_read_b128(smem + 2 * buf * kTileB + (k_lane ^ (ks << 5)) + tb * 32 * Tile::kRowB);
+  };
+  auto v_frag = [&](int buf, int st, int mb) -> u32x4 {
+    const char* vp = smem + (2 * buf + 1) * kTileB + v_lane + st * 16 * Tile::kRowB + ((mb << 6) ^ v_swz);
+    const u32x2 lo = lds_read_tr(vp), hi = lds_read_tr(vp + 8 * Tile::kRowB);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  // soft cap and mask of tile t's raw scores (a wave-uniform branch, which most tiles pass by)
+  auto finish_scores = [&](int t, f32x16 (&s)[NB]) {
+    if constexpr (CAP) {
+#pragma unroll
+      for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float e = fd_exp2(s[tb][i] * cap_in);
+          s[tb][i] = __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(1.0f + e), cap);   // tanh(y) = 1 - 2 / (1 + e^2y)
+        }
+    }
+    const int t0 = t * BN + wt * NT;       // first token of this wave's part
+    if (t0 + NT > wave_lo) {
+      const int see = my_limit - t0 - 4 * half;
+#pragma unroll
+      for (int tb = 0; tb < NB; ++tb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[tb][i] = tb * 32 + 8 * (i / 4) + i % 4 < see ? s[tb][i] : -INFINITY;
     }
   };
 
   f32x16 o[MB];
   float m, l;
-  bool careful = false;
-  for (;;) {
+  auto start = [&] {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) o[mb] = f32x16{};
     m = -3.0e38f;     // below every score: a row that sees nothing keeps l = 0
     l = 0.f;
-    int entry = 0;
-    if (t_first < t_last) {
-      const int rows0 = pool_row(t_first, page_entry(t_first));
-      request(0, rows0);
-      if (t_first + 1 < t_last) entry = page_entry(t_first + 1);
-      deposit(0);
+  };
+  // the reference point follows the maximum `mx` of the next tile's raw scores (this lane's tokens of its row)
+  auto move_reference = [&](float mx) {
+    const float top = fmaxf(m, half_max(mx) * c);
+    const float m_new = top - m > 8.0f ? top : m;
+    if (__any(m_new > m)) {
+      const float alpha = fd_exp2(m - m_new);
+      l *= alpha;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) o[mb] *= alpha;
+      m = m_new;
     }
+  };
+
+  // One tile of the pipelined walk.  On entry `cur` holds tile t's finished scores, `mx` their maximum over this lane, pr
+  // the pool rows of tile t + 1, whose K is on its way, like V of tile t.  The scores of tile t + 1 are computed while the
+  // weights of tile t are (one MFMA and a few weights at a time: the matrix pipe works on one while the vector pipe does
+  // the others), and their maximum while V of tile t is multiplied.
+  constexpr int E = 16 * NB;               // scores of a lane
+  auto step = [&](int t, int& entry, float& mx, f32x16 (&cur)[NB], f32x16 (&nxt)[NB], auto next_tag) {
+    constexpr bool NEXT = decltype(next_tag)::value;
+    const int buf = (t - t_first) & 1;
+    publish();
+    const bool more = NEXT && t + 2 < t_last;
+    if constexpr (NEXT) {
+      request(false, buf ^ 1);             // V of t + 1 over V of t - 1
+      if (more) {
+        rows_of(pool_row(t + 2, entry));
+        entry = page_entry(t + 3);
+        request(true, buf);                // K of t + 2 over K of t
+      }
+    }
+    move_reference(mx);
+    // P is rounded to the query's type for the second product (the sum l is not): half a step, 2^-8 (bf16) or 2^-11 (fp16)
+    // of each weight, of both signs -- less in their sum than the rounding of the output itself
+    u32x4 pf[NT / 16];
+    float sum0 = 0.f, sum1 = 0.f;
+    auto weights = [&](int e0, int e1) {   // scores e0 .. e1 - 1, in pairs
+#pragma unroll
+      for (int e = e0; e < e1; e += 2) {
+        const float p0 = fd_exp2(__builtin_fmaf(cur[e / 16][e % 16], c, -m));
+        const float p1 = fd_exp2(__builtin_fmaf(cur[e / 16][e % 16 + 1], c, -m));
+        sum0 += p0;
+        sum1 += p1;
+        pf[e / 8][e % 8 / 2] = Mma<T>::pack(p0, p1);
+      }
+    };
+    if constexpr (NEXT) {
+#pragma unroll
+      for (int tb = 0; tb < NB; ++tb) nxt[tb] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) nxt[tb] = Mma32<T>::run(k_frag(buf ^ 1, ks, tb), qf[ks], nxt[tb]);
+        weights(E * ks / KS & ~1, E * (ks + 1) / KS & ~1);
+      }
+      // pinned here: left to itself the compiler moves the weights behind the branches of finish_scores, next to their use
+#pragma unroll
+      for (int st = 0; st < NT / 16; ++st) asm volatile("" : "+v"(pf[st]));
+      l += sum0 + sum1;
+      asm volatile("" : "+v"(l));
+      finish_scores(t + 1, nxt);
+    } else {
+      weights(0, E);
+      l += sum0 + sum1;
+    }
+    mx = -INFINITY;
+#pragma unroll
+    for (int st = 0; st < NT / 16; ++st)
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        o[mb] = Mma32<T>::run(v_frag(buf, st, mb), pf[st], o[mb]);
+        if constexpr (NEXT) {
+          constexpr int N = NT / 16 * MB;  // MFMAs of this product
+          const int at = st * MB + mb;
+#pragma unroll
+          for (int e = E * at / N; e < E * (at + 1) / N; ++e) mx = fmaxf(mx, nxt[e / 16][e % 16]);
+        }
+      }
+    if constexpr (FP8 && NEXT) {
+      deposit(false, buf ^ 1);
+      if (more) deposit(true, buf);
+    }
+  };
+
+  auto walk = [&] {
+    start();
+    if (t_first >= t_last) return;
+    rows_of(pool_row(t_first, page_entry(t_first)));
+    int entry = page_entry(t_first + 1);
+    request(true, 0);
+    request(false, 0);
+    if constexpr (FP8) {
+      deposit(true, 0);
+      deposit(false, 0);
+    }
+    publish();
+    if (t_first + 1 < t_last) {
+      rows_of(pool_row(t_first + 1, entry));
+      entry = page_entry(t_first + 2);
+      request(true, 1);
+    }
+    f32x16 s0[NB], s1[NB];
+#pragma unroll
+    for (int tb = 0; tb < NB; ++tb) s0[tb] = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int tb = 0; tb < NB; ++tb) s0[tb] = Mma32<T>::run(k_frag(0, ks, tb), qf[ks], s0[tb]);
+    finish_scores(t_first, s0);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) mx = fmaxf(mx, s0[e / 16][e % 16]);
+    if constexpr (FP8) {
+      if (t_first + 1 < t_last) deposit(true, 1);
+    }
+    int t = t_first;
+    for (; t + 2 < t_last; t += 2) {       // two tiles a turn: the two sets of scores change places without copies
+      step(t, entry, mx, s0, s1, std::true_type{});
+      step(t + 1, entry, mx, s1, s0, std::true_type{});
+    }
+    if (t + 1 < t_last) {
+      step(t, entry, mx, s0, s1, std::true_type{});
+      step(t + 1, entry, mx, s1, s0, std::false_type{});
+    } else {
+      step(t, entry, mx, s0, s1, std::false_type{});
+    }
+  };
+
+  // The second walk of a workgroup whose result was not finite: tile by tile, no pipeline.
+  auto walk_careful = [&] {
+    start();
     for (int t = t_first; t < t_last; ++t) {
-      const int buf = (t - t_first) & 1;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();      // tile t is in LDS, and nobody reads the other buffer any more
-      if (t + 1 < t_last) {
-        const int next = pool_row(t + 1, entry);
-        if (t + 2 < t_last) entry = page_entry(t + 2);
-        request(buf ^ 1, next);
+      rows_of(pool_row(t, page_entry(t)));
+      __syncthreads();
+      request(true, 0);
+      request(false, 0);
+      deposit(true, 0);
+      deposit(false, 0);
+      publish();
+      f32x16 s[NB];
+#pragma unroll
+      for (int tb = 0; tb < NB; ++tb) s[tb] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int tb = 0; tb < NB; ++tb) s[tb] = Mma32<T>::run(k_frag(0, ks, tb), qf[ks], s[tb]);
+      finish_scores(t, s);
+      const int t0 = t * BN + wt * NT;
+      const bool masked = t0 + NT > wave_lo;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < E; ++e) mx = fmaxf(mx, s[e / 16][e % 16]);
+      move_reference(mx);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s[e / 16][e % 16] = fd_exp2(__builtin_fmaf(s[e / 16][e % 16], c, -m));
+        l += s[e / 16][e % 16];
       }
-      const int t0 = t * BN + wt * NT;       // first token of this wave's part
-      if (t0 < wave_hi) {
-        const char* kt = smem + buf * 2 * kTileB;
-        const char* vt = smem + buf * 2 * kTileB + kTileB + v_lane;
-        f32x16 s[NB];
 #pragma unroll
-        for (int tb = 0; tb < NB; ++tb) {
-          s[tb] = f32x16{};
+      for (int st = 0; st < NT / 16; ++st) {
+        u32x4 pf;
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const u32x4 kf = lds_read_b128(kt + (k_lane ^ (ks << 5)) + tb * 32 * Tile::kRowB);
-            s[tb] = Mma32<T>::run(kf, qf[ks], s[tb]);
-          }
-        }
-        if (a.soft_cap > 0.f) {
+        for (int w = 0; w < 4; ++w)
+          pf[w] = Mma<T>::pack(s[st / 2][8 * (st % 2) + 2 * w], s[st / 2][8 * (st % 2) + 2 * w + 1]);
+#pragma unroll 1
+        for (int mb = 0; mb < MB; ++mb) {
+          u32x4 vf = v_frag(0, st, mb);
+          if (masked) {
 #pragma unroll
-          for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = fd_exp2(2.0f * FD_LOG2E * s[tb][i] * cap_in);
-              s[tb][i] = cap * (1.0f - 2.0f / (1.0f + e));
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t e = vf[w] & Mma32<T>::kExp;
+              if ((e & 0xffffu) == (Mma32<T>::kExp & 0xffffu)) vf[w] &= 0xffff0000u;
+              if ((e >> 16) == (Mma32<T>::kExp >> 16)) vf[w] &= 0xffffu;
             }
-        }
-        const bool masked = t0 + NT > wave_lo;
-        if (masked) {
-          const int see = my_limit - t0 - 4 * half;
-#pragma unroll
-          for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              s[tb][i] = tb * 32 + 8 * (i / 4) + i % 4 < see ? s[tb][i] : -INFINITY;
-        }
-        float mx = s[0][0];
-#pragma unroll
-        for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
-        mx = half_max(mx) * c;
-        const float top = fmaxf(m, mx);
-        const float m_new = top - m > 8.0f ? top : m;
-        if (__any(m_new > m)) {
-          const float alpha = fd_exp2(m - m_new);
-          l *= alpha;
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) o[mb] *= alpha;
-          m = m_new;
-        }
-        float sum = 0.f;
-#pragma unroll
-        for (int tb = 0; tb < NB; ++tb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            s[tb][i] = fd_exp2(__builtin_fmaf(s[tb][i], c, -m));
-            sum += s[tb][i];
           }
-        l += sum;
-        // P is rounded to the query's type for the second product (the sum l is not): half a step, 2^-9 (bf16) or 2^-12
-        // (fp16) of each weight, below the rounding of the output itself
 #pragma unroll
-        for (int st = 0; st < NT / 16; ++st) {
-          u32x4 pf;
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            pf[w] = Mma<T>::pack(s[st / 2][8 * (st % 2) + 2 * w], s[st / 2][8 * (st % 2) + 2 * w + 1]);
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
-            const char* vp = vt + st * 16 * Tile::kRowB + ((mb << 6) ^ v_swz);
-            const u32x2 lo = lds_read_tr(vp), hi = lds_read_tr(vp + 8 * Tile::kRowB);
-            u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
-            if (careful && masked) {
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const uint32_t e = vf[w] & Mma32<T>::kExp;
-                if ((e & 0xffffu) == (Mma32<T>::kExp & 0xffffu)) vf[w] &= 0xffff0000u;
-                if ((e >> 16) == (Mma32<T>::kExp >> 16)) vf[w] &= 0xffffu;
-              }
-            }
-            o[mb] = Mma32<T>::run(vf, pf, o[mb]);
-          }
-        }
-        if (careful && masked) {
-          // the non-finite V values of this tile, for the rows that see them: lane (row, half) owns dims
-          // 32 mb + 8 i + 4 half .. + 3
-          for (int n = 0; n < NT; ++n) {
-            if (t0 + n >= my_limit) continue;
-            const int r = wt * NT + n;
-            const char* vr = smem + buf * 2 * kTileB + kTileB + r * Tile::kRowB;
-#pragma unroll
-            for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d0 = 32 * mb + 8 * i + 4 * half;
-                const u32x2 w = *(const u32x2*)(vr + ((((d0 >> 3) ^ Tile::v_swz(r)) << 4) | ((d0 & 4) << 1)));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint16_t bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                  if ((bits & (uint16_t)Mma32<T>::kExp) == (uint16_t)Mma32<T>::kExp)
-                    o[mb][4 * i + e] += (float)__builtin_bit_cast(T, bits);
-                }
-              }
-          }
+          for (int k = 0; k < MB; ++k)     // (registers have no run-time index)
+            if (k == mb) o[k] = Mma32<T>::run(vf, pf, o[k]);
         }
       }
-      if (t + 1 < t_last) deposit(buf ^ 1);
+      if (!masked) continue;
+      // the non-finite V values of this tile, for the rows that see them: lane (row, half) owns dims 32 mb + 8 i + 4 half
+      // .. + 3
+      for (int n = 0; n < NT; ++n) {
+        if (t0 + n >= my_limit) continue;
+        const int r = wt * NT + n;
+        const char* vr = smem + kTileB + r * Tile::kRowB;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d0 = 32 * mb + 8 * i + 4 * half;
+            const u32x2 w = *(const u32x2*)(vr + ((((d0 >> 3) ^ Tile::v_swz(r)) << 4) | ((d0 & 4) << 1)));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint16_t bits = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+              if ((bits & (uint16_t)Mma32<T>::kExp) == (uint16_t)Mma32<T>::kExp)
+                o[mb][4 * i + e] += (float)__builtin_bit_cast(T, bits);
+            }
+          }
+      }
     }
-    if (careful || t_first == t_last) break;
+  };
+  walk();
+  if (t_first < t_last) {
     // any value that is not finite?  (x - x is 0 for finite x)
     float probe = l - l;
 #pragma unroll
@@ -425,8 +532,7 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
     __syncthreads();
     const bool again = *flag != 0;
     __syncthreads();
-    if (!again) break;
-    careful = true;
+    if (again) walk_careful();
   }
 
   // ---- join the token groups, store
@@ -497,7 +603,7 @@ int launch_prefill(hipStream_t stream, const PrefillArgs& a) {
   const int64_t wgs = tiles * a.splits * a.Hkv;
   if (wgs >= ((int64_t)1 << 31)) return FD_ERR_TOO_LARGE;
   if (wgs == 0) return FD_OK;
-  auto kern = fd_prefill_kernel<T, FP8, D, WR, WT, BN>;
+  auto kern = a.soft_cap > 0.f ? fd_prefill_kernel<T, FP8, true, D, WR, WT, BN> : fd_prefill_kernel<T, FP8, false, D, WR, WT, BN>;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * WR * WT), lds, stream, a);
   return hipGetLastError() == hipSuccess ? FD_OK : FD_ERR_LAUNCH;
 }

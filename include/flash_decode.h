@@ -563,8 +563,8 @@ FD_API int fd_prefill(void* stream, const fd_prefill_args* args);
  * One decode step of sequences that share prefixes.  Group g is the sequences group_starts[g] .. group_starts[g + 1] - 1;
  * all of them attend to the prefix_lens[g] tokens of row g of prefix_table, and each of them to its own kv_lens[b] tokens
  * of block_table behind that (0 is allowed, for either).  A prefix is read once for its group: its part is a matrix product
- * of all the group's rows (fd_prefill's kernel), the sequences' own tokens go through the decode kernel, and one launch
- * merges the partials of both by their LSEs.  A sequence outside every group attends to its own tokens only.
+ * of all the group's rows (fd_prefill's kernel); the sequences' own tokens are further items of the same launch, and a second
+ * one merges the partials by their LSEs.  A sequence outside every group attends to its own tokens only.
  * `step` is the decode step over the sequences' own tokens as for fd_decode_planned, with combine_mode FD_COMBINE_SPLIT and
  * without extra partials, seq_order and flags; its workspace is the whole step's (fd_decode_shared_workspace_bytes).
  * 16-bit queries, caches of the same type or fp8, equal K and V head dims.

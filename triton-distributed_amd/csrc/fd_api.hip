@@ -1205,44 +1205,49 @@ namespace {
 
 constexpr int kMaxPrefillSplits = 64;
 
+int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
+
 struct PrefillPlan {
   int row_groups;             // 32-row groups of a workgroup's tile: 1, 2 or 4
-  int splits;                 // key ranges per row tile
+  int splits, min_tiles;      // key ranges per row tile, of at least so many tiles
   int64_t part_bytes, lse_off, total;
 };
 
+// Ranges that `items` work items of up to `key_tiles` key tiles each are cut into.  Up to one workgroup per CU a range may be
+// as short as two tiles (such calls are latency); the second workgroup that a CU has room for (64 KB of LDS each) has to
+// bring eight tiles, or the partials cost more than it gains: 64 sequences behind a prefix of 8192 tokens 22.8 us + 14.3 us
+// of merge with 32 ranges of 4 tiles, 23.8 + 9.4 us with 16 of 8; but 128 sequences in four groups with prefixes of up to
+// 16384 tokens 71 us with 8 ranges of 32 tiles, 102 us with 4.  *min_tiles: the same bound for sequences shorter than planned.
+int plan_ranges(int64_t items, int64_t key_tiles, int head_dim, int* min_tiles) {
+  *min_tiles = 1;
+  if (items <= 0) return 1;
+  const int64_t first = min64(256 / items, key_tiles / 2);
+  const int64_t second = head_dim == 256 ? 0 : min64(512 / items, key_tiles / 8);
+  int64_t s = first > second ? first : second;
+  if (s > kMaxPrefillSplits) s = kMaxPrefillSplits;
+  if (s <= 1) return 1;
+  *min_tiles = second >= first ? 8 : 2;
+  return (int)s;
+}
+
 // Row tile and key ranges from what the host knows: sizes, not lengths.  `rows` query rows (tokens) in `batch` sequences,
-// `tokens` keys in the longest.
-//  * Row tile: 128 rows of a KV head (token, head pairs) where a sequence has more than 64 on average; below that the waves
-//    of a workgroup share the keys of 64 or 32 rows instead of idling on rows that do not exist.
-//  * Key ranges: two workgroups fit a CU (one with head_dim 256); a grid that leaves half of those places empty is cut
-//    along the keys, as long as a range keeps four tiles, and the partials are merged by a second launch.
+// `tokens` keys in the longest.  Row tile: 128 rows of a KV head (token, head pairs) where a sequence has more than 64 on
+// average; below that the waves of a workgroup share the keys of 64 or 32 rows instead of idling on rows that do not exist.
 void plan_prefill(const fd_params* p, int32_t batch, int64_t rows, int64_t tokens, int want_splits, PrefillPlan* pl) {
   const int G = p->q_heads / p->kv_heads;
   const int64_t avg = batch > 0 ? (rows * G + batch - 1) / batch : 0;
   pl->row_groups = avg <= 32 && p->head_dim != 256 ? 1 : avg <= 64 ? 2 : 4;
   const int bm = 32 * pl->row_groups;
   const int bn = p->head_dim == 256 ? 32 : 64;
-  const int64_t places = p->head_dim == 256 ? 256 : 512;
   int64_t tiles = (rows * G + bm - 1) / bm;
   if (tiles < batch) tiles = batch;
-  int64_t s = want_splits;
-  if (s <= 0) {
-    s = 1;
-    const int64_t items = tiles * p->kv_heads;
-    if (items > 0 && 2 * items <= places) {
-      s = places / items;
-      const int64_t most = (tokens + bn - 1) / bn / 4;
-      if (s > most) s = most;
-      if (s > kMaxPrefillSplits) s = kMaxPrefillSplits;
-      if (s < 1) s = 1;
-    }
-  }
-  pl->splits = (int)s;
-  const int64_t lines = rows * p->q_heads * s;
-  pl->part_bytes = s > 1 ? lines * p->head_dim * 4 : 0;
+  pl->min_tiles = 1;
+  pl->splits = want_splits > 0 ? want_splits
+                               : plan_ranges(tiles * p->kv_heads, (tokens + bn - 1) / bn, p->head_dim, &pl->min_tiles);
+  const int64_t lines = rows * p->q_heads * pl->splits;
+  pl->part_bytes = pl->splits > 1 ? lines * p->head_dim * 4 : 0;
   pl->lse_off = align256(pl->part_bytes);
-  pl->total = s > 1 ? pl->lse_off + align256(lines * 4) : 0;
+  pl->total = pl->splits > 1 ? pl->lse_off + align256(lines * 4) : 0;
 }
 
 // Everything about a row-tile launch that does not depend on pointers.
@@ -1313,6 +1318,9 @@ int fill_prefill(const char* fn, const fd_prefill_args* a, PrefillArgs* k) {
   if (!aligned16(a->k) || !aligned16(a->v) || a->stride_k_tok % kv16 || a->stride_k_h % kv16 ||
       a->stride_v_tok % kv16 || a->stride_v_h % kv16)
     return fail(FD_ERR_ALIGNMENT, "%s: K/V rows must be 16-byte aligned (pointer and token/head strides)", fn);
+  const int64_t widest = (((int64_t)1 << 31) - 1) / (fp8 ? 1 : 2);
+  if (a->stride_k_tok < 0 || a->stride_v_tok < 0 || a->stride_k_tok > widest || a->stride_v_tok > widest)
+    return fail(FD_ERR_INVALID_ARG, "%s: token stride out of range", fn);
   if ((reinterpret_cast<uintptr_t>(a->out) & 7) || a->stride_ot % 4 || a->stride_oh % 4)
     return fail(FD_ERR_ALIGNMENT, "%s: output rows must be 8-byte aligned (pointer and token/head strides)", fn);
   memset(k, 0, sizeof(*k));
@@ -1346,13 +1354,13 @@ int check_workspace(const char* fn, const void* ws, int64_t have, int64_t need, 
   return FD_OK;
 }
 
-// Plan of a shared-prefix step: the decode step over the sequences' own tokens (fp32 partials, every slot written) and the
-// row tiles over the prefixes, one workspace for both.
+// Plan of a shared-prefix step: row tiles over the prefixes and the sequences' own keys are items of one launch, the
+// partials of both lie next to each other.
 struct SharedPlan {
-  StepPlan step;
-  PrefillPlan rows;
+  PrefillPlan rows;           // of the groups
   fd_params prefix;
-  int64_t own_off, own_lse_off, order_off, total;
+  int own_splits, own_min_tiles;
+  int64_t lse_off, total;
 };
 
 int plan_shared(const char* fn, const fd_shared_args* a, SharedPlan* sp) {
@@ -1364,25 +1372,22 @@ int plan_shared(const char* fn, const fd_shared_args* a, SharedPlan* sp) {
       a->step.combine_mode != FD_COMBINE_SPLIT)
     return fail(FD_ERR_INVALID_ARG, "%s: a step without flags, extra partials, order or rank merge, in FD_COMBINE_SPLIT", fn);
   if (p->out_dtype != p->q_dtype) return fail(FD_ERR_UNSUPPORTED, "%s: the output has the query's type", fn);
-  sp->prefix = *p;
+  fd_params own = *p;
+  own.num_splits = 0;
+  if (int rc = check_prefill_shape(fn, &own, batch, batch, true)) return rc;
+  sp->prefix = own;
   sp->prefix.max_pages_per_seq = a->prefix_max_pages > 0 ? a->prefix_max_pages : 1;
   sp->prefix.max_kv_len = a->max_prefix_len;
-  sp->prefix.num_splits = 0;
   if (int rc = check_prefill_shape(fn, &sp->prefix, batch, batch, true)) return rc;
-  if (int rc = plan_step(fn, p, batch, 1, 0, false, &sp->step)) return rc;
-  sp->step.p.mid_dtype = FD_F32;
-  const int64_t tokens = planned_tokens(&sp->prefix);
-  plan_prefill(&sp->prefix, a->groups, batch, tokens, 0, &sp->rows);
-  // the prefix part always leaves partials: there are the sequences' own to merge with
-  const int64_t lines = (int64_t)batch * p->q_heads;
-  const int D = p->head_dim;
-  sp->rows.part_bytes = lines * sp->rows.splits * D * 4;
-  sp->rows.lse_off = align256(sp->rows.part_bytes);
-  sp->own_off = sp->rows.lse_off + align256(lines * sp->rows.splits * 4);
-  const int64_t own = lines * sp->step.p.num_splits;
-  sp->own_lse_off = sp->own_off + align256(own * D * 4);
-  sp->order_off = sp->own_lse_off + align256(own * 4);
-  sp->total = sp->order_off + align256(sp->step.order_bytes);
+  plan_prefill(&sp->prefix, a->groups, batch, planned_tokens(&sp->prefix), 0, &sp->rows);
+  // the sequences' own keys fill the chip on their own terms: they run next to the prefixes where those leave room
+  const int bm = 32 * sp->rows.row_groups, bn = p->head_dim == 256 ? 32 : 64;
+  const int64_t tiles = (p->q_heads / p->kv_heads + bm - 1) / bm;
+  sp->own_splits = plan_ranges((int64_t)batch * tiles * p->kv_heads, (planned_tokens(&own) + bn - 1) / bn, p->head_dim,
+                               &sp->own_min_tiles);
+  const int64_t lines = (int64_t)batch * p->q_heads * (sp->rows.splits + sp->own_splits);
+  sp->lse_off = align256(lines * p->head_dim * 4);
+  sp->total = sp->lse_off + align256(lines * 4);
   return FD_OK;
 }
 
@@ -1406,17 +1411,14 @@ int fd_prefill(void* stream, const fd_prefill_args* a) {
   if (int rc = fill_prefill(fn, a, &k)) return rc;
   if (int rc = check_workspace(fn, a->workspace, a->workspace_bytes, pl.total, 256)) return rc;
   k.splits = pl.splits;
+  k.min_tiles = pl.min_tiles;
   if (pl.splits > 1) {
     k.part = (float*)a->workspace;
     k.part_lse = (float*)((char*)a->workspace + pl.lse_off);
   }
   if (int rc = launch_rows(fn, stream, k, &a->params, pl.row_groups)) return rc;
   if (pl.splits == 1) return FD_OK;
-  PrefillMergeArgs m;
-  memset(&m, 0, sizeof(m));
-  m.rows = k;
-  m.out_dtype = a->params.q_dtype;
-  const int rc = fd_launch_prefill_merge((hipStream_t)stream, m, a->params.head_dim);
+  const int rc = fd_launch_prefill_merge((hipStream_t)stream, k, a->params.head_dim, a->params.q_dtype);
   if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
   return FD_OK;
 }
@@ -1442,15 +1444,13 @@ int fd_decode_shared(void* stream, const fd_shared_args* a) {
   if (!st->kv_lens || !st->block_table) return fail(FD_ERR_INVALID_ARG, "%s: NULL tensor pointer", fn);
   if (int rc = check_workspace(fn, st->workspace, st->workspace_bytes, sp.total, 256)) return rc;
   char* ws = (char*)st->workspace;
-  const int D = st->params.head_dim;
 
-  // the prefixes: the sequences of a group are the rows of its tile, without a causal limit
+  // the sequences of a group are the rows of its tiles, without a causal limit
   fd_prefill_args pa;
   memset(&pa, 0, sizeof(pa));
   pa.q = st->q; pa.k = st->k_cache; pa.v = st->v_cache; pa.out = st->out; pa.lse_out = st->lse_out;
-  // (without groups the row-tile kernel is not launched; the pointers only have to pass the checks)
   pa.cu_seqlens_q = a->group_starts;
-  pa.kv_lens = a->groups ? a->prefix_lens : st->kv_lens;
+  pa.kv_lens = a->groups ? a->prefix_lens : st->kv_lens;           // (without groups the pointers only pass the checks)
   pa.block_table = a->groups ? a->prefix_table : st->block_table;
   pa.stride_q_t = st->stride_q_bs; pa.stride_q_h = st->stride_q_h; pa.stride_k_tok = st->stride_k_tok;
   pa.stride_k_h = st->stride_k_h; pa.stride_v_tok = st->stride_v_tok; pa.stride_v_h = st->stride_v_h;
@@ -1459,36 +1459,17 @@ int fd_decode_shared(void* stream, const fd_shared_args* a) {
   PrefillArgs k;
   if (int rc = fill_prefill(fn, &pa, &k)) return rc;
   k.splits = sp.rows.splits;
+  k.min_tiles = sp.rows.min_tiles;
   k.part = (float*)ws;
-  k.part_lse = (float*)(ws + sp.rows.lse_off);
-
-  // the sequences' own tokens
-  const int32_t* order = nullptr;
-  if (sp.step.order_kind != FD_ORDER_NONE) {
-    int32_t* o = (int32_t*)(ws + sp.order_off);
-    const int rc = sp.step.order_kind == FD_ORDER_ITEMS ? fd_schedule_items(stream, st->kv_lens, st->batch, o, &sp.step.p)
-                                                        : fd_schedule(stream, st->kv_lens, st->batch, o);
-    if (rc != FD_OK) return rc;
-    order = o;
-  }
-  if (a->groups > 0) {
-    if (int rc = launch_rows(fn, stream, k, &sp.prefix, sp.rows.row_groups)) return rc;
-  }
-  const int64_t S1 = sp.step.p.num_splits;
-  if (int rc = split_impl(fn, stream, st->q, st->k_cache, st->v_cache, ws + sp.own_off, (float*)(ws + sp.own_lse_off),
-                          st->sm_scale, st->block_table, st->kv_lens, st->batch, st->stride_q_bs, st->stride_q_h,
-                          st->stride_k_tok, st->stride_k_h, st->stride_v_tok, st->stride_v_h,
-                          (int64_t)st->params.q_heads * S1 * D, S1 * D, D, st->stride_table_bs, order, &sp.step.p, nullptr,
-                          nullptr))
-    return rc;
-  PrefillMergeArgs m;
-  memset(&m, 0, sizeof(m));
-  m.rows = k;
-  m.part1 = (const float*)(ws + sp.own_off);
-  m.part1_lse = (const float*)(ws + sp.own_lse_off);
-  m.S1 = (int)S1;
-  m.out_dtype = st->params.out_dtype;
-  const int rc = fd_launch_prefill_merge((hipStream_t)stream, m, D);
+  k.part_lse = (float*)(ws + sp.lse_off);
+  k.own_lens = st->kv_lens;
+  k.own_bt = st->block_table;
+  k.own_sbt = st->stride_table_bs;
+  k.own_splits = sp.own_splits;
+  k.own_min_tiles = sp.own_min_tiles;
+  k.own_max_pages = st->params.max_pages_per_seq;
+  if (int rc = launch_rows(fn, stream, k, &sp.prefix, sp.rows.row_groups)) return rc;
+  const int rc = fd_launch_prefill_merge((hipStream_t)stream, k, st->params.head_dim, st->params.out_dtype);
   if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
   return FD_OK;
 }

@@ -120,8 +120,8 @@ struct PrefillArgs {
   const void* v;
   void* out;
   float* lse;                // nullptr or [total_q, Hq]
-  float* part;               // nullptr (one split: out and lse), or fp32 partials [total_q, Hq, splits, D]
-  float* part_lse;           // ... and their LSEs [total_q, Hq, splits]
+  float* part;               // nullptr (one split: out and lse), or fp32 partials [total_q, Hq, splits + own_splits, D]
+  float* part_lse;           // ... and their LSEs [total_q, Hq, splits + own_splits]
   const int32_t* cu_q;       // [batch + 1], or nullptr: batch == 1, all rows
   const int32_t* q_lens;     // nullptr, or [batch]: rows of a sequence behind its first q_lens are padding
   const int32_t* cu_k;       // packed keys: [batch + 1]
@@ -131,18 +131,17 @@ struct PrefillArgs {
   const float* v_scale;
   int64_t sq_t, sq_h, sk_t, sk_h, sv_t, sv_h, so_t, so_h, sbt;
   float sm_scale, soft_cap;
-  int32_t batch, total_q, total_k, Hq, Hkv, G, P, max_pages, num_pages, causal, splits;
-  uint32_t p_magic, p_shift;  // n / P
-  uint32_t g_magic, g_shift;  // n / G
-};
-
-// Arguments of the merge of two lists of partials per row (fd_prefill_merge.hip).
-struct PrefillMergeArgs {
-  PrefillArgs rows;          // rows, spans and outputs; part / part_lse / splits: the first list
-  const float* part1;        // nullptr, or the second list [total_q, Hq, S1, D] fp32, which every row has: rows outside the
-                             // spans are then merged from it alone instead of being left as they are
-  const float* part1_lse;    // [total_q, Hq, S1]
-  int32_t S1, out_dtype;
+  int32_t batch, total_q, total_k, Hq, Hkv, G, P, max_pages, num_pages, causal;
+  int32_t splits, min_tiles; // key ranges per row tile, of at least min_tiles tiles
+  uint32_t p_magic, p_shift; // n / P
+  uint32_t g_magic, g_shift; // n / G
+  // Shared-prefix step (own_splits > 0): batch counts the groups, whose rows are sequences, and every row has keys of its
+  // own besides: own_lens[row] tokens of row `row` of own_bt, in own_splits ranges.  Their work items come behind the
+  // first `group_units` (row tile, range) items of the groups.
+  const int32_t* own_lens;
+  const int32_t* own_bt;
+  int64_t own_sbt;
+  int32_t own_splits, own_min_tiles, own_max_pages, group_units;
 };
 
 // A pair of page pools [layers, pages, P, heads, dim]; a page is contiguous, strides in bytes.
@@ -1270,7 +1269,7 @@ int fd_launch_kv_append(hipStream_t stream, const AppendArgs& a, int src_dtype, 
 int fd_launch_prefill_d64(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
 int fd_launch_prefill_d128(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
 int fd_launch_prefill_d256(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
-int fd_launch_prefill_merge(hipStream_t stream, const PrefillMergeArgs& a, int head_dim);
+int fd_launch_prefill_merge(hipStream_t stream, const PrefillArgs& a, int head_dim, int out_dtype);
 int fd_launch_pages_copy(hipStream_t stream, const PagePool& pool, const int32_t* src, const int32_t* dst, int n);
 int fd_launch_pages_reserve(hipStream_t stream, const PageTables& t, int num_pages, int page_size,
                             const int32_t* new_tokens, int uniform, int32_t* ok);

@@ -121,47 +121,71 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const int half = lane >> 5, l32 = lane & 31;
 
   // ---- work item: KV head fastest (the eight XCDs take neighbouring workgroups in turn, so with eight KV heads each
-  // XCD's L2 holds one head's keys), then the split, then the row tile
+  // XCD's L2 holds one head's keys), then the key range, then the row tile
   const int kvh = blockIdx.x % a.Hkv;
-  const int rest = blockIdx.x / a.Hkv;
-  const int split = rest % a.splits;
-  const int tile = rest / a.splits;
-  int b = -1, q_start = 0, n_q = 0, j = 0;
-  {
-    int base = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 64) {
-      int s = 0, n = 0;
-      if (b0 + lane < a.batch) fd_prefill_span(a, b0 + lane, s, n);
-      const int tiles = (n * a.G + BM - 1) / BM;
-      int incl = tiles;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int up = __shfl_up(incl, off);
-        if (lane >= off) incl += up;
+  int unit = blockIdx.x / a.Hkv, slot, split, splits, min_tiles;     // slot: of the partial
+  int b = -1, q_start = 0, n_q = 0, k_start = 0, n_k = 0, j = 0;
+  const int32_t* table = a.bt;
+  if (a.own_splits > 0 && unit >= a.group_units) {
+    // a sequence's own keys behind its group's prefix
+    unit -= a.group_units;
+    splits = a.own_splits;
+    min_tiles = a.own_min_tiles;
+    split = unit % splits;
+    slot = a.splits + split;
+    const int rest = unit / splits, tiles = (a.G + BM - 1) / BM;
+    q_start = rest / tiles;
+    j = rest - q_start * tiles;
+    if (q_start >= a.total_q) return;
+    n_q = 1;
+    n_k = min(max(a.own_lens[q_start], 0), a.own_max_pages * a.P);
+    table = a.own_bt + (int64_t)q_start * a.own_sbt;
+  } else {
+    splits = a.splits;
+    min_tiles = a.min_tiles;
+    split = slot = unit % splits;
+    const int tile = unit / splits;
+    // The row tile of the list: sequences with the most keys first (in blocks of 64 sequences, one a lane), the tiles of a
+    // sequence from its end, where a causal row sees the most -- short work fills in behind long.  In index order the last
+    // long sequence of a batch runs alone at the end.
+    for (int b0 = 0, base = 0; b0 < a.batch; b0 += 64) {
+      const int mine = b0 + lane;
+      int qs = 0, nq = 0, ks = 0, nk = -1, tiles = 0;
+      if (mine < a.batch) {
+        fd_prefill_span(a, mine, qs, nq);
+        if (a.bt) {
+          nk = min(max(a.kv_lens[mine], 0), a.max_pages * a.P);
+        } else {
+          ks = min(max(a.cu_k[mine], 0), a.total_k);
+          nk = min(max(a.cu_k[mine + 1], ks), a.total_k) - ks;
+        }
+        tiles = (nq * a.G + BM - 1) / BM;
       }
-      const uint64_t past = __ballot(base + incl > tile);
-      if (past) {
-        const int at = __builtin_ctzll(past);
-        b = b0 + at;
-        q_start = __builtin_amdgcn_readlane(s, at);
-        n_q = __builtin_amdgcn_readlane(n, at);
-        const int mine = __builtin_amdgcn_readlane(tiles, at);
-        // the tiles of a sequence from its end: in the causal form the ones with the most keys first
-        j = mine - 1 - (tile - base - (__builtin_amdgcn_readlane(incl, at) - mine));
+      int before = 0, total = 0;                // tiles of the sequences that come before this lane's; of all
+      const int n = min(64, a.batch - b0);
+      for (int i = 0; i < n; ++i) {
+        const int k_i = __builtin_amdgcn_readlane(nk, i), t_i = __builtin_amdgcn_readlane(tiles, i);
+        before += k_i > nk || (k_i == nk && i < lane) ? t_i : 0;
+        total += t_i;
+      }
+      const int at = tile - base - before;
+      const uint64_t here = __ballot(at >= 0 && at < tiles);
+      if (here) {
+        const int w = __builtin_ctzll(here);
+        b = b0 + w;
+        q_start = __builtin_amdgcn_readlane(qs, w);
+        n_q = __builtin_amdgcn_readlane(nq, w);
+        k_start = __builtin_amdgcn_readlane(ks, w);
+        n_k = __builtin_amdgcn_readlane(nk, w);
+        j = __builtin_amdgcn_readlane(tiles, w) - 1 - __builtin_amdgcn_readlane(at, w);
         break;
       }
-      base += __builtin_amdgcn_readlane(incl, 63);
+      base += total;
     }
+    if (b < 0) return;
+    if (table) table += (int64_t)b * a.sbt;
   }
-  if (b < 0) return;
 
-  int n_k, k_start = 0;
-  if (a.bt) {
-    n_k = min(max(a.kv_lens[b], 0), a.max_pages * a.P);
-  } else {
-    k_start = min(max(a.cu_k[b], 0), a.total_k);
-    n_k = min(max(a.cu_k[b + 1], k_start), a.total_k) - k_start;
-  }
   const int rows = n_q * a.G;
   // keys that row r of the sequence sees: [0, limit)
   auto token_of = [&](int r) { return (int)(((uint64_t)(uint32_t)r * a.g_magic) >> a.g_shift); };
@@ -174,7 +198,7 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const int wave_lo = limit_of(min(r0 + wr * 32, rows - 1));            // the wave's rows see at least this many keys
   const int wg_hi = limit_of(min(r0 + BM - 1, rows - 1));
   const int all_tiles = (max(wg_hi, 0) + BN - 1) / BN;
-  const int per_split = (all_tiles + a.splits - 1) / a.splits;
+  const int per_split = max((all_tiles + splits - 1) / splits, min_tiles);
   const int t_first = min(split * per_split, all_tiles);
   const int t_last = min(t_first + per_split, all_tiles);
 
@@ -211,7 +235,6 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const char* kb = (const char*)a.k + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sk_h);
   const char* vb = (const char*)a.v + (FP8 ? 1 : 2) * ((int64_t)kvh * a.sv_h);
   const uint32_t sk_b = (uint32_t)a.sk_t * (FP8 ? 1 : 2), sv_b = (uint32_t)a.sv_t * (FP8 ? 1 : 2);
-  const int32_t* table = a.bt ? a.bt + (int64_t)b * a.sbt : nullptr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
 
   // The token row in the pool of token t0 + lane of a tile (lanes past BN repeat the last): page entry first, so that it
@@ -441,6 +464,38 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
     }
   };
 
+  // A wave whose rows are all past the end only fetches.
+  auto walk_idle = [&] {
+    start();
+    if (t_first >= t_last) return;
+    rows_of(pool_row(t_first, page_entry(t_first)));
+    int entry = page_entry(t_first + 1);
+    request(true, 0);
+    request(false, 0);
+    deposit(true, 0);
+    deposit(false, 0);
+    publish();
+    if (t_first + 1 < t_last) {
+      rows_of(pool_row(t_first + 1, entry));
+      entry = page_entry(t_first + 2);
+      request(true, 1);
+      deposit(true, 1);
+    }
+    for (int t = t_first; t < t_last; ++t) {
+      const int buf = (t - t_first) & 1;
+      publish();
+      if (t + 1 >= t_last) continue;
+      request(false, buf ^ 1);
+      if (t + 2 < t_last) {
+        rows_of(pool_row(t + 2, entry));
+        entry = page_entry(t + 3);
+        request(true, buf);
+      }
+      deposit(false, buf ^ 1);
+      if (t + 2 < t_last) deposit(true, buf);
+    }
+  };
+
   // The second walk of a workgroup whose result was not finite: tile by tile, no pipeline.
   auto walk_careful = [&] {
     start();
@@ -516,7 +571,7 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
       }
     }
   };
-  walk();
+  if (r0 + wr * 32 < rows) walk(); else walk_idle();
   if (t_first < t_last) {
     // any value that is not finite?  (x - x is 0 for finite x)
     float probe = l - l;
@@ -571,10 +626,10 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
   const int64_t tok = q_start + q_tok;
   const int head = kvh * a.G + q_head;
   if (a.part) {
-    const int64_t pr = (tok * a.Hq + head) * a.splits + split;
-    if (half == 0) a.part_lse[pr] = lse;
+    const int64_t at = (tok * a.Hq + head) * (a.splits + a.own_splits) + slot;
+    if (half == 0) a.part_lse[at] = lse;
     if (l == 0.f) return;         // weight 0: the row is not looked at
-    float* dst = a.part + pr * D;
+    float* dst = a.part + at * D;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
@@ -596,13 +651,16 @@ __global__ void __launch_bounds__(64 * WR * WT, D == 256 ? 1 : 2) fd_prefill_ker
 }
 
 template <typename T, bool FP8, int D, int WR, int WT, int BN>
-int launch_prefill(hipStream_t stream, const PrefillArgs& a) {
+int launch_prefill(hipStream_t stream, const PrefillArgs& args) {
+  PrefillArgs a = args;
   constexpr int BM = 32 * WR;
   constexpr size_t lds = 4 * BN * 2 * D;
   const int64_t tiles = ((int64_t)a.total_q * a.G + (int64_t)a.batch * (BM - 1)) / BM;   // sum of ceil(rows_b / BM) at most
-  const int64_t wgs = tiles * a.splits * a.Hkv;
+  const int64_t own = a.own_splits > 0 ? (int64_t)a.total_q * ((a.G + BM - 1) / BM) * a.own_splits : 0;
+  const int64_t wgs = (tiles * a.splits + own) * a.Hkv;
   if (wgs >= ((int64_t)1 << 31)) return FD_ERR_TOO_LARGE;
   if (wgs == 0) return FD_OK;
+  a.group_units = (int32_t)(tiles * a.splits);
   auto kern = a.soft_cap > 0.f ? fd_prefill_kernel<T, FP8, true, D, WR, WT, BN> : fd_prefill_kernel<T, FP8, false, D, WR, WT, BN>;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(64 * WR * WT), lds, stream, a);
   return hipGetLastError() == hipSuccess ? FD_OK : FD_ERR_LAUNCH;

@@ -19,11 +19,12 @@ from typing import Optional, Union
 
 import torch
 
-from .._lib import FdPagePool, FdPageTables, check, load_library, stream_handle
-from .prefill import _check_devices, _check_int32, _need, _new, _on_device_of
+from .._lib import FdPagePool, FdPageTables, load_library
+from .prefill import _check_devices, _check_int32, _launch, _need, _new, _remember, _sig
 
 
 def _pool(name, k_cache, v_cache) -> FdPagePool:
+    """The pools' shape, checked; the addresses are the call's."""
     _need(k_cache.dim() in (4, 5) and v_cache.dim() == k_cache.dim() and k_cache.shape[:-2] == v_cache.shape[:-2],
           f"{name}: pools [pages, P, heads, dim] or [layers, pages, P, heads, dim] with the same pages")
     p = FdPagePool()
@@ -34,7 +35,6 @@ def _pool(name, k_cache, v_cache) -> FdPagePool:
         _need(t.stride(-1) == 1 and (heads == 1 or t.stride(-2) == dim) and (rows == 1 or t.stride(-3) == heads * dim),
               f"{name}: a page must be contiguous")
         size = t.element_size()
-        setattr(p, side + "_cache", t.data_ptr())
         setattr(p, side + "_layer_stride", (t.stride(0) if t.dim() == 5 else 0) * size)
         # (a single page has no distance to a next one)
         setattr(p, side + "_page_stride", (t.stride(-4) if p.num_pages > 1 else rows * heads * dim) * size)
@@ -48,32 +48,49 @@ def _tables(name, block_table, kv_lens, page_refs, num_pages) -> FdPageTables:
           f"{name}: block_table must be int32 [B, max_pages] with contiguous rows")
     _check_int32(name, "page_refs", page_refs, (num_pages,))
     t = FdPageTables()
-    t.block_table, t.page_refs, t.stride_table_bs = block_table.data_ptr(), page_refs.data_ptr(), block_table.stride(0)
+    t.stride_table_bs = block_table.stride(0)
     t.batch, t.max_pages_per_seq = block_table.shape
     if kv_lens is not None:
         _check_int32(name, "kv_lens", kv_lens, (block_table.shape[0],))
-        t.kv_lens = kv_lens.data_ptr()
     return t
 
 
-def _run(fn, ref, stream, *args):
-    with _on_device_of(ref):
-        rc = fn(stream_handle(stream, ref.device.index), *args)
-    if rc:
-        check(rc)
+_SEEN = {}   # pool and table images of calls whose arguments have been checked, by what the checks look at
+
+
+def _checked(name, caches, tables, lists):
+    """(fd_page_pool, fd_page_tables) of a call, checked once per kind of arguments.  caches: (k_cache, v_cache) or ();
+    tables: (block_table, kv_lens or None, page_refs) or (); lists: further int32 tensors as (what, tensor, shape)."""
+    key = (name, *map(_sig, caches), *map(_sig, tables), *((w, _sig(t), s) for w, t, s in lists))
+    images = _SEEN.get(key)
+    if images is None:
+        _check_devices(name, *caches, *tables, *(t for _, t, _ in lists))
+        pool = _pool(name, *caches) if caches else None
+        for what, t, shape in lists:
+            if t is not None:
+                _check_int32(name, what, t, shape)
+        pages = pool.num_pages if caches else tables[2].numel()
+        images = _remember(_SEEN, key, (bytes(pool) if caches else None,
+                                        bytes(_tables(name, *tables, pages)) if tables else None))
+    pool = t = None
+    if caches:
+        pool = FdPagePool.from_buffer_copy(images[0])
+        pool.k_cache, pool.v_cache = caches[0].data_ptr(), caches[1].data_ptr()
+    if tables:
+        t = FdPageTables.from_buffer_copy(images[1])
+        t.block_table, t.page_refs = tables[0].data_ptr(), tables[2].data_ptr()
+        if tables[1] is not None:
+            t.kv_lens = tables[1].data_ptr()
+    return pool, t
 
 
 def paged_kv_copy(k_cache, v_cache, src_pages, dst_pages, *, stream=None):
     """Copies page ``src_pages[i]`` to page ``dst_pages[i]`` (int32 ``[n]``) in every layer of both pools.  The destinations
     must be distinct and none of them a source; ids outside the pool are skipped."""
-    name = "paged_kv_copy"
-    _check_devices(name, k_cache, v_cache, src_pages, dst_pages)
-    pool = _pool(name, k_cache, v_cache)
     n = src_pages.numel()
-    _check_int32(name, "src_pages", src_pages, (n,))
-    _check_int32(name, "dst_pages", dst_pages, (n,))
+    pool, _ = _checked("paged_kv_copy", (k_cache, v_cache), (), (("src_pages", src_pages, (n,)), ("dst_pages", dst_pages, (n,))))
     if n:
-        _run(load_library().fd_pages_copy, k_cache, stream, byref(pool), src_pages.data_ptr(), dst_pages.data_ptr(), n)
+        _launch(load_library().fd_pages_copy, k_cache.device, stream, byref(pool), src_pages.data_ptr(), dst_pages.data_ptr(), n)
 
 
 def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, torch.Tensor], page_size: int, *,
@@ -82,21 +99,17 @@ def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, tor
     the append that follows has somewhere to write.  Returns int32 ``[B]``: 1, or 0 where the table is too narrow or the
     pool has run out -- that row keeps what it had.  Rows are served in order; a row that gets nothing still counts against
     the rows behind it.  At most 4096 rows."""
-    name = "paged_kv_reserve"
     each = new_tokens if isinstance(new_tokens, torch.Tensor) else None
-    _check_devices(name, block_table, kv_lens, page_refs, each, ok_out)
-    t = _tables(name, block_table, kv_lens, page_refs, page_refs.numel())
-    _need(t.batch <= 4096, f"{name}: {t.batch} rows (at most 4096)")
-    if each is not None:
-        _check_int32(name, "new_tokens", each, (t.batch,))
-    else:
-        _need(0 <= new_tokens < 1 << 31, f"{name}: new_tokens {new_tokens}")
+    batch = block_table.shape[0]
+    _, t = _checked("paged_kv_reserve", (), (block_table, kv_lens, page_refs),
+                    (("new_tokens", each, (batch,)), ("ok_out", ok_out, (batch,))))
     if ok_out is None:
-        ok_out = _new(t.batch, torch.int32, block_table.device, stream)
-    _check_int32(name, "ok_out", ok_out, (t.batch,))
-    if t.batch:
-        _run(load_library().fd_pages_reserve, block_table, stream, byref(t), page_refs.numel(), int(page_size),
-             each.data_ptr() if each is not None else None, 0 if each is not None else int(new_tokens), ok_out.data_ptr())
+        ok_out = _new(batch, torch.int32, block_table.device, stream)
+    _need(batch <= 4096, f"paged_kv_reserve: {batch} rows (at most 4096)")
+    _need(each is not None or 0 <= new_tokens < 1 << 31, f"paged_kv_reserve: new_tokens {new_tokens}")
+    if batch:
+        _launch(load_library().fd_pages_reserve, block_table.device, stream, byref(t), page_refs.numel(), int(page_size),
+                each.data_ptr() if each is not None else None, 0 if each is not None else int(new_tokens), ok_out.data_ptr())
     return ok_out
 
 
@@ -107,35 +120,27 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
     afterwards.  Returns int32 ``[n]``: 1, or 0 where a fork is refused and nothing changes (a row out of range or its own
     parent, a child that holds tokens or pages or was named before, no free page left).  Parents count as they are before
     the call."""
-    name = "paged_kv_fork"
-    _check_devices(name, k_cache, v_cache, block_table, kv_lens, page_refs, parents, children, ok_out)
-    pool = _pool(name, k_cache, v_cache)
-    t = _tables(name, block_table, kv_lens, page_refs, pool.num_pages)
     n = parents.numel()
-    _check_int32(name, "parents", parents, (n,))
-    _check_int32(name, "children", children, (n,))
+    pool, t = _checked("paged_kv_fork", (k_cache, v_cache), (block_table, kv_lens, page_refs),
+                       (("parents", parents, (n,)), ("children", children, (n,)), ("ok_out", ok_out, (n,))))
     if ok_out is None:
         ok_out = _new(n, torch.int32, k_cache.device, stream)
-    _check_int32(name, "ok_out", ok_out, (n,))
     if n:
         lib = load_library()
         need = lib.fd_pages_workspace_bytes(pool.num_pages, n)
         ws = _new(need, torch.uint8, k_cache.device, stream)
-        _run(lib.fd_pages_fork, k_cache, stream, byref(pool), byref(t), parents.data_ptr(), children.data_ptr(), n,
-             ok_out.data_ptr(), ws.data_ptr(), need)
+        _launch(lib.fd_pages_fork, k_cache.device, stream, byref(pool), byref(t), parents.data_ptr(), children.data_ptr(), n,
+                ok_out.data_ptr(), ws.data_ptr(), need)
     return ok_out
 
 
 def paged_kv_free(block_table, kv_lens, page_refs, rows, *, stream=None):
     """Takes their pages from the listed rows (int32 ``[n]``): counts go down -- a page that no row holds any more is free --,
     the rows' entries become -1 and their lengths 0.  Empty rows, rows listed twice and rows out of range are skipped."""
-    name = "paged_kv_free"
-    _check_devices(name, block_table, kv_lens, page_refs, rows)
-    t = _tables(name, block_table, kv_lens, page_refs, page_refs.numel())
     n = rows.numel()
-    _check_int32(name, "rows", rows, (n,))
+    _, t = _checked("paged_kv_free", (), (block_table, kv_lens, page_refs), (("rows", rows, (n,)),))
     if n and t.batch:
-        _run(load_library().fd_pages_free, block_table, stream, byref(t), page_refs.numel(), rows.data_ptr(), n)
+        _launch(load_library().fd_pages_free, block_table.device, stream, byref(t), page_refs.numel(), rows.data_ptr(), n)
 
 
 def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Optional[torch.Tensor] = None,
@@ -143,15 +148,11 @@ def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Opti
     """Moves the live pages to the front of the pool, in every layer: with ``n`` live pages, the k-th live page at or behind
     ``n`` goes to the k-th free page before ``n``; ``page_refs`` and ``block_table`` follow.  ``block_table`` must hold every
     row that holds pages.  Returns int32 ``[1]`` (on the device): ``n``, from where on the pool is free."""
-    name = "paged_kv_compact"
-    _check_devices(name, k_cache, v_cache, block_table, page_refs, live_out)
-    pool = _pool(name, k_cache, v_cache)
-    t = _tables(name, block_table, None, page_refs, pool.num_pages)
+    pool, t = _checked("paged_kv_compact", (k_cache, v_cache), (block_table, None, page_refs), (("live_out", live_out, (1,)),))
     if live_out is None:
         live_out = _new(1, torch.int32, k_cache.device, stream)
-    _check_int32(name, "live_out", live_out, (1,))
     lib = load_library()
     need = lib.fd_pages_workspace_bytes(pool.num_pages, 0)
     ws = _new(need, torch.uint8, k_cache.device, stream)
-    _run(lib.fd_pages_compact, k_cache, stream, byref(pool), byref(t), live_out.data_ptr(), ws.data_ptr(), need)
+    _launch(lib.fd_pages_compact, k_cache.device, stream, byref(pool), byref(t), live_out.data_ptr(), ws.data_ptr(), need)
     return live_out

@@ -12,7 +12,6 @@ only: a query, key or value that requires a gradient is refused while autograd r
 """
 from __future__ import annotations
 
-import contextlib
 from ctypes import byref
 from typing import Optional
 
@@ -47,10 +46,9 @@ def _check_scales(name, k_scale, v_scale, kv_heads):
               f"{name}: fp8 scales are contiguous float32 tensors of {kv_heads} values")
 
 
-def _check_no_grad(name, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            _need(not t.requires_grad, f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
+def _check_no_grad(name, q, k, v):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
 
 
 def _check_pool(name, q, k_cache, v_cache):
@@ -71,11 +69,20 @@ def _check_table(name, what, table, rows):
           f"{name}: {what} must be int32 [{rows}, max_pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
 
 
-def _on_device_of(t):
-    """The device whose kernels and streams a call uses is the tensors', whatever the current one is."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(fn, device, stream, *args):
+    """Calls the library on the tensors' device, whatever the current one is, and raises what it reports."""
+    if device.index == torch.cuda.current_device():
+        rc = fn(stream_handle(stream, device.index), *args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(stream_handle(stream, device.index), *args)
+    if rc:
+        check(rc)
+
+
+def _sig(t):
+    """What the checks of an argument look at: a call whose arguments have all been seen before skips them."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def _new(shape, dtype, device, stream):
@@ -134,34 +141,53 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     library choose how many key ranges a row tile is cut into (more than one where there are few rows), else exactly that
     many, up to 64.
     """
-    name = "gqa_fwd_batch_prefill"
-    a, need, output = _prefill_args(name, q, k, v, cu_seqlens_q, kv_lens, block_table, scale, soft_cap, causal, cu_seqlens_k,
-                                    q_lens, output, lse_out, k_scale, v_scale, max_kv_len, kv_split, stream, True)
-    if q.shape[0] == 0 or a.batch == 0:
+    _check_no_grad("gqa_fwd_batch_prefill", q, k, v)
+    key = (_sig(q), _sig(k), _sig(v), _sig(cu_seqlens_q), _sig(kv_lens), _sig(block_table), _sig(cu_seqlens_k), _sig(q_lens),
+           _sig(output), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, causal, max_kv_len, kv_split)
+    cached = _PREFILL_CACHE.get(key)
+    if cached is None:
+        cached = _remember(_PREFILL_CACHE, key, _prefill_image(
+            "gqa_fwd_batch_prefill", q, k, v, cu_seqlens_q, kv_lens, block_table, scale, soft_cap, causal, cu_seqlens_k,
+            q_lens, output, lse_out, k_scale, v_scale, max_kv_len, kv_split))
+    image, need = cached
+    if output is None:
+        output = _new(q.shape, q.dtype, q.device, stream)
+    if image is None:      # no rows, or no sequence
         return output
-    lib = load_library()
-    hold = _workspace(workspace, need, q.device, stream)
-    if hold is not None:
+    a = FdPrefillArgs.from_buffer_copy(image)
+    a.q = q_ptr = q.data_ptr()
+    # (an empty tensor has no address: nothing is read through the stand-in)
+    a.k, a.v = k.data_ptr() or q_ptr, v.data_ptr() or q_ptr
+    a.cu_seqlens_q, a.out = cu_seqlens_q.data_ptr(), output.data_ptr()
+    if lse_out is not None:
+        a.lse_out = lse_out.data_ptr()
+    if q_lens is not None:
+        a.q_lens = q_lens.data_ptr()
+    if block_table is not None:
+        a.block_table, a.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
+    else:
+        a.cu_seqlens_k = (cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k).data_ptr()
+    if k_scale is not None:
+        a.params.k_scale, a.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    if need:
+        hold = _workspace(workspace, need, q.device, stream)
         a.workspace, a.workspace_bytes = hold.data_ptr(), need
-    with _on_device_of(q):
-        rc = lib.fd_prefill(stream_handle(stream, q.device.index), byref(a))
-    if rc:
-        check(rc)
+    _launch(load_library().fd_prefill, q.device, stream, byref(a))
     return output
 
 
 def prefill_workspace_bytes(q, k, v, cu_seqlens_q, kv_lens, block_table, *, cu_seqlens_k=None, k_scale=None, v_scale=None,
                             max_kv_len=None, kv_split=0) -> int:
     """Bytes of workspace that ``gqa_fwd_batch_prefill`` uses for tensors of these shapes (0: none)."""
-    return _prefill_args("prefill_workspace_bytes", q, k, v, cu_seqlens_q, kv_lens, block_table, 1.0, 0.0, True,
-                         cu_seqlens_k, None, None, None, k_scale, v_scale, max_kv_len, kv_split, None, False)[1]
+    return _prefill_image("prefill_workspace_bytes", q, k, v, cu_seqlens_q, kv_lens, block_table, 1.0, 0.0, True,
+                          cu_seqlens_k, None, None, None, k_scale, v_scale, max_kv_len, kv_split)[1]
 
 
-def _prefill_args(name, q, k, v, cu_q, kv_lens, block_table, scale, soft_cap, causal, cu_k, q_lens, output, lse_out, k_scale,
-                  v_scale, max_kv_len, kv_split, stream, with_output):
+def _prefill_image(name, q, k, v, cu_q, kv_lens, block_table, scale, soft_cap, causal, cu_k, q_lens, output, lse_out,
+                   k_scale, v_scale, max_kv_len, kv_split):
+    """Checks a call and returns (the fd_prefill_args image without its pointers, bytes of workspace)."""
     _need(q.dim() == 3 and q.stride(2) == 1, f"{name}: q must be [total_q, Hq, D] with a contiguous last dim")
     _check_devices(name, q, k, v, cu_q, kv_lens, block_table, cu_k, q_lens, output, lse_out, k_scale, v_scale)
-    _check_no_grad(name, q, k, v)
     _need(cu_q.dim() == 1 and cu_q.numel() >= 1, f"{name}: cu_seqlens_q must be int32 [batch + 1]")
     batch = cu_q.numel() - 1
     _check_int32(name, "cu_seqlens_q", cu_q, (batch + 1,))
@@ -190,55 +216,28 @@ def _prefill_args(name, q, k, v, cu_q, kv_lens, block_table, scale, soft_cap, ca
     _check_scales(name, k_scale, v_scale, kv_heads)
     if q_lens is not None:
         _check_int32(name, "q_lens", q_lens, (batch,))
-    if with_output:
-        if output is None:
-            output = _new(q.shape, q.dtype, q.device, stream)
-        _need(output.shape == q.shape and output.dtype == q.dtype and output.stride(2) == 1,
-              f"{name}: output must have the query's shape and type and a contiguous last dim")
-        _need(lse_out is None or (lse_out.dtype == torch.float32 and tuple(lse_out.shape) == (total_q, q_heads)
-                                  and lse_out.is_contiguous()),
-              f"{name}: lse_out must be a contiguous float32 tensor [{total_q}, {q_heads}]")
-    o_st = output.stride()[:2] if output is not None else (0, 0)
-    key = (q.shape, q.stride(), q.dtype, k.shape, k_st, v_st, k.dtype, batch, paged, max_pages, table_st, o_st, scale,
-           soft_cap, causal, k_scale is not None, max_kv_len, kv_split)
-    cached = _PREFILL_CACHE.get(key)
-    if cached is None:
-        a = FdPrefillArgs()
-        a.stride_q_t, a.stride_q_h = q.stride()[:2]
-        (a.stride_k_tok, a.stride_k_h), (a.stride_v_tok, a.stride_v_h) = k_st, v_st
-        a.stride_ot, a.stride_oh = o_st
-        a.stride_table_bs, a.sm_scale, a.batch, a.total_q, a.total_k = table_st, float(scale), batch, total_q, total_k
-        a.causal = 1 if causal else 0
-        p = a.params
-        p.q_heads, p.kv_heads, p.head_dim, p.page_size, p.num_pages = q_heads, kv_heads, head_dim, page_size, num_pages
-        p.max_pages_per_seq, p.q_dtype, p.kv_dtype = max_pages, fd_dtype_of(q), fd_dtype_of(k, fp8_bytes=k_scale is not None)
-        p.out_dtype, p.soft_cap = p.q_dtype, float(soft_cap or 0.0)
-        p.max_kv_len, p.num_splits = int(max_kv_len or 0), int(kv_split)
-        probe = FdPrefillArgs.from_buffer_copy(a)
-        probe.block_table = 256 if paged else None    # whether there is a table is all that the size asks of it
-        need = load_library().fd_prefill_workspace_bytes(byref(probe))
-        if need < 0:
-            check(int(need))
-        cached = _remember(_PREFILL_CACHE, key, (bytes(a), need))
-    image, need = cached
-    a = FdPrefillArgs.from_buffer_copy(image)
-    a.q = q.data_ptr()
-    # (an empty tensor has no address: nothing is read through the stand-in)
-    a.k, a.v = k.data_ptr() or a.q, v.data_ptr() or a.q
-    a.cu_seqlens_q = cu_q.data_ptr()
-    if output is not None:
-        a.out = output.data_ptr()
-    if lse_out is not None:
-        a.lse_out = lse_out.data_ptr()
-    if q_lens is not None:
-        a.q_lens = q_lens.data_ptr()
-    if paged:
-        a.block_table, a.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
-    else:
-        a.cu_seqlens_k = cu_k.data_ptr()
-    if k_scale is not None:
-        a.params.k_scale, a.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-    return a, need, output
+    _need(output is None or (output.shape == q.shape and output.dtype == q.dtype and output.stride(2) == 1),
+          f"{name}: output must have the query's shape and type and a contiguous last dim")
+    _need(lse_out is None or (lse_out.dtype == torch.float32 and tuple(lse_out.shape) == (total_q, q_heads)
+                              and lse_out.is_contiguous()),
+          f"{name}: lse_out must be a contiguous float32 tensor [{total_q}, {q_heads}]")
+    a = FdPrefillArgs()
+    a.stride_q_t, a.stride_q_h = q.stride()[:2]
+    a.stride_ot, a.stride_oh = output.stride()[:2] if output is not None else (q_heads * head_dim, head_dim)
+    (a.stride_k_tok, a.stride_k_h), (a.stride_v_tok, a.stride_v_h) = k_st, v_st
+    a.stride_table_bs, a.sm_scale, a.batch, a.total_q, a.total_k = table_st, float(scale), batch, total_q, total_k
+    a.causal = 1 if causal else 0
+    p = a.params
+    p.q_heads, p.kv_heads, p.head_dim, p.page_size, p.num_pages = q_heads, kv_heads, head_dim, page_size, num_pages
+    p.max_pages_per_seq, p.q_dtype, p.kv_dtype = max_pages, fd_dtype_of(q), fd_dtype_of(k, fp8_bytes=k_scale is not None)
+    p.out_dtype, p.soft_cap = p.q_dtype, float(soft_cap or 0.0)
+    p.max_kv_len, p.num_splits = int(max_kv_len or 0), int(kv_split)
+    probe = FdPrefillArgs.from_buffer_copy(a)
+    probe.block_table = 256 if paged else None    # whether there is a table is all that the size asks of it
+    need = load_library().fd_prefill_workspace_bytes(byref(probe))
+    if need < 0:
+        check(int(need))
+    return (bytes(a) if total_q and batch else None), need
 
 
 def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, prefix_lens,
@@ -258,11 +257,44 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     group's query heads.  ``q_lens`` is accepted and ignored, ``workspace`` used if it is large enough, as there; 16-bit
     queries with a cache of the same type or fp8-e4m3.  ``max_kv_len`` / ``max_prefix_len``: host-side hints.
     """
-    name = "gqa_fwd_batch_decode_shared_prefix"
+    _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache)
+    # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
+    hints = (-(-max_kv_len // 1024) * 1024 if max_kv_len else 0, -(-max_prefix_len // 1024) * 1024 if max_prefix_len else 0)
+    key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(kv_lens), _sig(block_table), _sig(prefix_lens), _sig(prefix_table),
+           _sig(group_starts), _sig(output_combine), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, hints)
+    cached = _SHARED_CACHE.get(key)
+    if cached is None:
+        cached = _remember(_SHARED_CACHE, key, _shared_image(
+            "gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache, kv_lens, block_table, prefix_lens, prefix_table, scale,
+            soft_cap, group_starts, output_combine, lse_out, k_scale, v_scale, hints))
+    image, need = cached
+    if output_combine is None:
+        output_combine = _new(q.shape, q.dtype, q.device, stream)
+    if image is None:      # no sequence
+        return output_combine
+    a = FdSharedArgs.from_buffer_copy(image)
+    s = a.step
+    hold = _workspace(workspace, need, q.device, stream)
+    s.workspace, s.workspace_bytes = hold.data_ptr(), need
+    s.q, s.k_cache, s.v_cache, s.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output_combine.data_ptr()
+    s.block_table, s.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
+    a.prefix_table, a.prefix_lens = prefix_table.data_ptr(), prefix_lens.data_ptr()
+    if group_starts is not None:
+        a.group_starts = group_starts.data_ptr()
+    if lse_out is not None:
+        s.lse_out = lse_out.data_ptr()
+    if k_scale is not None:
+        s.params.k_scale, s.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    _launch(load_library().fd_decode_shared, q.device, stream, byref(a))
+    return output_combine
+
+
+def _shared_image(name, q, k_cache, v_cache, kv_lens, block_table, prefix_lens, prefix_table, scale, soft_cap, group_starts,
+                  output_combine, lse_out, k_scale, v_scale, hints):
+    """Checks a call and returns (the fd_shared_args image without its pointers, bytes of workspace)."""
     _need(q.dim() == 3 and q.stride(2) == 1, f"{name}: q must be [B, Hq, D] with a contiguous last dim")
     _check_devices(name, q, k_cache, v_cache, kv_lens, block_table, prefix_lens, prefix_table, group_starts, output_combine,
                    lse_out, k_scale, v_scale)
-    _check_no_grad(name, q, k_cache, v_cache)
     _check_pool(name, q, k_cache, v_cache)
     batch, q_heads, head_dim = q.shape
     kv_heads = k_cache.shape[2]
@@ -277,55 +309,28 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
         _need(groups == 1, f"{name}: {groups} prefixes need group_starts")
     else:
         _check_int32(name, "group_starts", group_starts, (groups + 1,))
-    if output_combine is None:
-        output_combine = _new(q.shape, q.dtype, q.device, stream)
-    _need(output_combine.shape == q.shape and output_combine.dtype == q.dtype and output_combine.stride(2) == 1,
+    _need(output_combine is None or (output_combine.shape == q.shape and output_combine.dtype == q.dtype
+                                     and output_combine.stride(2) == 1),
           f"{name}: output_combine must have the query's shape and type and a contiguous last dim")
     _need(lse_out is None or (lse_out.dtype == torch.float32 and lse_out.numel() == batch * q_heads
                               and lse_out.is_contiguous()), f"{name}: lse_out must be contiguous float32 [{batch}, {q_heads}]")
     if batch == 0:
-        return output_combine
-    lib = load_library()
-    q_st, k_st, v_st, o_st = q.stride(), k_cache.stride(), v_cache.stride(), output_combine.stride()
-    # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
-    hints = tuple(-(-n // 1024) * 1024 if n else 0 for n in (max_kv_len, max_prefix_len))
-    key = (q.shape, q_st, q.dtype, k_cache.shape, k_st, v_st, k_cache.dtype, block_table.shape[1], block_table.stride(0),
-           prefix_table.shape, prefix_table.stride(0), o_st, scale, soft_cap, k_scale is not None, hints)
-    cached = _SHARED_CACHE.get(key)
-    if cached is None:
-        a = FdSharedArgs()
-        s = a.step
-        s.stride_q_bs, s.stride_q_h, s.stride_obs, s.stride_oh = q_st[0], q_st[1], o_st[0], o_st[1]
-        s.stride_k_tok, s.stride_k_h, s.stride_v_tok, s.stride_v_h = k_st[1], k_st[2], v_st[1], v_st[2]
-        s.stride_table_bs, s.sm_scale, s.batch, s.combine_mode = block_table.stride(0), float(scale), batch, FD_COMBINE_SPLIT
-        p: FdParams = s.params
-        p.q_heads, p.kv_heads, p.head_dim, p.page_size = q_heads, kv_heads, head_dim, k_cache.shape[1]
-        p.num_splits, p.num_pages, p.max_pages_per_seq = -1, k_cache.shape[0], block_table.shape[1]
-        p.q_dtype, p.kv_dtype = fd_dtype_of(q), fd_dtype_of(k_cache, fp8_bytes=k_scale is not None)
-        p.out_dtype, p.soft_cap, p.max_kv_len = p.q_dtype, float(soft_cap or 0.0), hints[0]
-        a.stride_prefix_bs, a.groups, a.prefix_max_pages = prefix_table.stride(0), groups, prefix_table.shape[1]
-        a.max_prefix_len = hints[1]
-        need = lib.fd_decode_shared_workspace_bytes(byref(a))
-        if need < 0:
-            check(int(need))
-        cached = _remember(_SHARED_CACHE, key, (bytes(a), need))
-    image, need = cached
-    a = FdSharedArgs.from_buffer_copy(image)
+        return None, 0
+    q_st, k_st, v_st = q.stride(), k_cache.stride(), v_cache.stride()
+    o_st = output_combine.stride() if output_combine is not None else (q_heads * head_dim, head_dim)
+    a = FdSharedArgs()
     s = a.step
-    hold = _workspace(workspace, need, q.device, stream)
-    s.workspace, s.workspace_bytes = hold.data_ptr(), need
-    s.q, s.k_cache, s.v_cache, s.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output_combine.data_ptr()
-    s.block_table, s.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
-    a.prefix_table, a.prefix_lens = prefix_table.data_ptr(), prefix_lens.data_ptr()
-    if group_starts is not None:
-        a.group_starts = group_starts.data_ptr()
-    if lse_out is not None:
-        s.lse_out = lse_out.data_ptr()
-    if k_scale is not None:
-        s.params.k_scale, s.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-    with _on_device_of(q):
-        rc = lib.fd_decode_shared(stream_handle(stream, q.device.index), byref(a))
-    if rc:
-        check(rc)
-    return output_combine
-
+    s.stride_q_bs, s.stride_q_h, s.stride_obs, s.stride_oh = q_st[0], q_st[1], o_st[0], o_st[1]
+    s.stride_k_tok, s.stride_k_h, s.stride_v_tok, s.stride_v_h = k_st[1], k_st[2], v_st[1], v_st[2]
+    s.stride_table_bs, s.sm_scale, s.batch, s.combine_mode = block_table.stride(0), float(scale), batch, FD_COMBINE_SPLIT
+    p: FdParams = s.params
+    p.q_heads, p.kv_heads, p.head_dim, p.page_size = q_heads, kv_heads, head_dim, k_cache.shape[1]
+    p.num_splits, p.num_pages, p.max_pages_per_seq = -1, k_cache.shape[0], block_table.shape[1]
+    p.q_dtype, p.kv_dtype = fd_dtype_of(q), fd_dtype_of(k_cache, fp8_bytes=k_scale is not None)
+    p.out_dtype, p.soft_cap, p.max_kv_len = p.q_dtype, float(soft_cap or 0.0), hints[0]
+    a.stride_prefix_bs, a.groups, a.prefix_max_pages = prefix_table.stride(0), groups, prefix_table.shape[1]
+    a.max_prefix_len = hints[1]
+    need = load_library().fd_decode_shared_workspace_bytes(byref(a))
+    if need < 0:
+        check(int(need))
+    return bytes(a), need

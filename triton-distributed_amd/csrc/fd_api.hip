@@ -1208,7 +1208,7 @@ constexpr int kMaxPrefillSplits = 64;
 int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 
 struct PrefillPlan {
-  int row_groups;             // 32-row groups of a workgroup's tile: 1, 2 or 4
+  bool row_tiles;             // tiles of 128 rows, else of 32
   int splits, min_tiles;      // key ranges per row tile, of at least so many tiles
   int64_t part_bytes, lse_off, total;
 };
@@ -1231,13 +1231,13 @@ int plan_ranges(int64_t items, int64_t key_tiles, int head_dim, int* min_tiles) 
 }
 
 // Row tile and key ranges from what the host knows: sizes, not lengths.  `rows` query rows (tokens) in `batch` sequences,
-// `tokens` keys in the longest.  Row tile: 128 rows of a KV head (token, head pairs) where a sequence has more than 64 on
-// average; below that the waves of a workgroup share the keys of 64 or 32 rows instead of idling on rows that do not exist.
+// `tokens` keys in the longest.  Row tile: 128 rows of a KV head (token, head pairs) where a sequence has more than 32 on
+// average; below that the waves of a workgroup share the keys of 32 rows instead of idling on rows that do not exist.
 void plan_prefill(const fd_params* p, int32_t batch, int64_t rows, int64_t tokens, int want_splits, PrefillPlan* pl) {
   const int G = p->q_heads / p->kv_heads;
   const int64_t avg = batch > 0 ? (rows * G + batch - 1) / batch : 0;
-  pl->row_groups = avg <= 32 && p->head_dim != 256 ? 1 : avg <= 64 ? 2 : 4;
-  const int bm = 32 * pl->row_groups;
+  pl->row_tiles = avg > 32;
+  const int bm = pl->row_tiles ? 128 : 32;
   const int bn = p->head_dim == 256 ? 32 : 64;
   int64_t tiles = (rows * G + bm - 1) / bm;
   if (tiles < batch) tiles = batch;
@@ -1277,7 +1277,7 @@ int check_prefill_shape(const char* fn, const fd_params* p, int32_t batch, int64
     if ((int64_t)p->num_pages * p->page_size >= (int64_t)1 << 31)
       return fail(FD_ERR_TOO_LARGE, "%s: pool of %lld token rows exceeds 2^31", fn,
                   (long long)p->num_pages * p->page_size);
-    if ((int64_t)p->max_pages_per_seq * p->page_size >= ((int64_t)1 << 31) - 256)
+    if ((int64_t)p->max_pages_per_seq * p->page_size > INT32_MAX - 1024)
       return fail(FD_ERR_TOO_LARGE, "%s: block table capacity exceeds 2^31 tokens", fn);
   }
   return FD_OK;
@@ -1288,6 +1288,7 @@ int check_prefill(const char* fn, const fd_prefill_args* a, PrefillPlan* pl) {
   const bool paged = a->block_table != nullptr;
   if (int rc = check_prefill_shape(fn, p, a->batch, a->total_q, paged)) return rc;
   if (!paged && a->total_k < 0) return fail(FD_ERR_INVALID_ARG, "%s: total_k %d", fn, a->total_k);
+  if (!paged && a->total_k > INT32_MAX - 1024) return fail(FD_ERR_TOO_LARGE, "%s: total_k %d", fn, a->total_k);
   // packed keys: the longest sequence is not known; all of them where there is one, else twice the average
   int64_t tokens;
   if (paged) {
@@ -1338,10 +1339,10 @@ int fill_prefill(const char* fn, const fd_prefill_args* a, PrefillArgs* k) {
   return FD_OK;
 }
 
-int launch_rows(const char* fn, void* stream, const PrefillArgs& k, const fd_params* p, int row_groups) {
+int launch_rows(const char* fn, void* stream, const PrefillArgs& k, const fd_params* p, bool row_tiles) {
   const bool fp8 = p->kv_dtype == FD_FP8_E4M3;
   auto launch = p->head_dim == 64 ? fd_launch_prefill_d64 : p->head_dim == 128 ? fd_launch_prefill_d128 : fd_launch_prefill_d256;
-  const int rc = launch((hipStream_t)stream, k, p->q_dtype, fp8, row_groups);
+  const int rc = launch((hipStream_t)stream, k, p->q_dtype, fp8, row_tiles);
   if (rc == FD_ERR_TOO_LARGE) return fail(rc, "%s: too many row tiles for one launch", fn);
   if (rc != FD_OK) return fail(rc, "%s: launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
   return FD_OK;
@@ -1381,8 +1382,8 @@ int plan_shared(const char* fn, const fd_shared_args* a, SharedPlan* sp) {
   if (int rc = check_prefill_shape(fn, &sp->prefix, batch, batch, true)) return rc;
   plan_prefill(&sp->prefix, a->groups, batch, planned_tokens(&sp->prefix), 0, &sp->rows);
   // the sequences' own keys fill the chip on their own terms: they run next to the prefixes where those leave room
-  const int bm = 32 * sp->rows.row_groups, bn = p->head_dim == 256 ? 32 : 64;
-  const int64_t tiles = (p->q_heads / p->kv_heads + bm - 1) / bm;
+  const int bn = p->head_dim == 256 ? 32 : 64;
+  const int64_t tiles = (p->q_heads / p->kv_heads + 31) / 32;
   sp->own_splits = plan_ranges((int64_t)batch * tiles * p->kv_heads, (planned_tokens(&own) + bn - 1) / bn, p->head_dim,
                                &sp->own_min_tiles);
   const int64_t lines = (int64_t)batch * p->q_heads * (sp->rows.splits + sp->own_splits);
@@ -1416,7 +1417,7 @@ int fd_prefill(void* stream, const fd_prefill_args* a) {
     k.part = (float*)a->workspace;
     k.part_lse = (float*)((char*)a->workspace + pl.lse_off);
   }
-  if (int rc = launch_rows(fn, stream, k, &a->params, pl.row_groups)) return rc;
+  if (int rc = launch_rows(fn, stream, k, &a->params, pl.row_tiles)) return rc;
   if (pl.splits == 1) return FD_OK;
   const int rc = fd_launch_prefill_merge((hipStream_t)stream, k, a->params.head_dim, a->params.q_dtype);
   if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
@@ -1468,7 +1469,7 @@ int fd_decode_shared(void* stream, const fd_shared_args* a) {
   k.own_splits = sp.own_splits;
   k.own_min_tiles = sp.own_min_tiles;
   k.own_max_pages = st->params.max_pages_per_seq;
-  if (int rc = launch_rows(fn, stream, k, &sp.prefix, sp.rows.row_groups)) return rc;
+  if (int rc = launch_rows(fn, stream, k, &sp.prefix, sp.rows.row_tiles)) return rc;
   const int rc = fd_launch_prefill_merge((hipStream_t)stream, k, st->params.head_dim, st->params.out_dtype);
   if (rc != FD_OK) return fail(rc, "%s: merge launch failed: %s", fn, hipGetErrorString(hipGetLastError()));
   return FD_OK;

@@ -1266,9 +1266,9 @@ int fd_launch_schedule(hipStream_t stream, const int32_t* kv_lens, int batch, in
 int fd_launch_schedule_items(hipStream_t stream, const int32_t* kv_lens, int batch, int64_t capacity,
                              const RangePlan& ranges, int32_t* items);
 int fd_launch_kv_append(hipStream_t stream, const AppendArgs& a, int src_dtype, int kv_dtype);
-int fd_launch_prefill_d64(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
-int fd_launch_prefill_d128(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
-int fd_launch_prefill_d256(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, int row_groups);
+int fd_launch_prefill_d64(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, bool row_tiles);
+int fd_launch_prefill_d128(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, bool row_tiles);
+int fd_launch_prefill_d256(hipStream_t stream, const PrefillArgs& a, int q_dtype, bool fp8, bool row_tiles);
 int fd_launch_prefill_merge(hipStream_t stream, const PrefillArgs& a, int head_dim, int out_dtype);
 int fd_launch_pages_copy(hipStream_t stream, const PagePool& pool, const int32_t* src, const int32_t* dst, int n);
 int fd_launch_pages_reserve(hipStream_t stream, const PageTables& t, int num_pages, int page_size,

@@ -141,7 +141,7 @@ struct PrefillArgs {
   const int32_t* own_lens;
   const int32_t* own_bt;
   int64_t own_sbt;
-  int32_t own_splits, own_min_tiles, own_max_pages, group_units;
+  int32_t own_splits, own_min_tiles, own_max_pages, group_units, own_units;
 };
 
 // A pair of page pools [layers, pages, P, heads, dim]; a page is contiguous, strides in bytes.

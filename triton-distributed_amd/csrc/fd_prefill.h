@@ -501,17 +501,18 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) pr[i] = __shfl(row, ((i * NW + wave) * 64 + lane) / W::kInChunks);
   };
+  auto request_one = [&](bool is_k, int buf, int i) {
+    const int n = (i * NW + wave) * 64 + lane;
+    const int r = n / W::kInChunks, ch = n % W::kInChunks;
+    const char* src = (is_k ? w.kb : w.vb) + (uint64_t)(uint32_t)pr[i] * (is_k ? w.sk_b : w.sv_b) + (W::source_chunk(is_k, r, ch) << 4);
+    if constexpr (FP8)
+      (is_k ? f8k : f8v)[i] = *(const u32x4*)src;
+    else
+      load_to_lds_b128(src, __builtin_amdgcn_readfirstlane(lds0 + (2 * buf + (is_k ? 0 : 1)) * kTileB + (i * NW + wave) * 1024));
+  };
   auto request = [&](bool is_k, int buf) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int n = (i * NW + wave) * 64 + lane;
-      const int r = n / W::kInChunks, ch = n % W::kInChunks;
-      const char* src = (is_k ? w.kb : w.vb) + (uint64_t)(uint32_t)pr[i] * (is_k ? w.sk_b : w.sv_b) + (W::source_chunk(is_k, r, ch) << 4);
-      if constexpr (FP8)
-        (is_k ? f8k : f8v)[i] = *(const u32x4*)src;
-      else
-        load_to_lds_b128(src, __builtin_amdgcn_readfirstlane(lds0 + (2 * buf + (is_k ? 0 : 1)) * kTileB + (i * NW + wave) * 1024));
-    }
+    for (int i = 0; i < kLoads; ++i) request_one(is_k, buf, i);
   };
   auto deposit = [&](bool is_k, int buf) {   // fp8: convert what `request` fetched and put it into LDS
     if constexpr (FP8) {
@@ -527,25 +528,17 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
     __syncthreads();
   };
 
-  // One tile of the pipelined walk.  On entry `cur` holds tile t's finished scores, `mx` their maximum over this lane, pr
-  // the pool rows of tile t + 1, whose K is on its way, like V of tile t.  The scores of tile t + 1 are computed while the
+  // One tile of the pipelined walk.  On entry `cur` holds tile t's finished scores, which the reference point
+  // has followed, pr the pool rows of tile t + 1, whose K is on its way, like V of tile t.  The scores of tile t + 1 are computed while the
   // weights of tile t are (one MFMA and a few weights at a time: the matrix pipe works on one while the vector pipe does
   // the others), and their maximum while V of tile t is multiplied.
-  auto fetch_next = [&](int t, int buf, int& entry) {
-    request(false, buf ^ 1);               // V of t + 1 over V of t - 1
-    if (t + 2 < t_last) {
-      rows_of(t + 2, entry);
-      entry = page_entry(t + 3);
-      request(true, buf);                  // K of t + 2 over K of t
-    }
-  };
+  constexpr int kEvery = KS / 2 / kLoads;  // k steps between two requests
+  static_assert(KS == 2 * kEvery * kLoads, "the requests fit under the scores");
   constexpr int E = 16 * NB;               // scores of a lane
-  auto step = [&](int t, int& entry, float& mx, f32x16 (&cur)[NB], f32x16 (&nxt)[NB], auto next_tag) {
+  auto step = [&](int t, int& entry, f32x16 (&cur)[NB], f32x16 (&nxt)[NB], auto next_tag) {
     constexpr bool NEXT = decltype(next_tag)::value;
     const int buf = (t - t_first) & 1;
     publish();
-    if constexpr (NEXT) fetch_next(t, buf, entry);
-    w.move_reference(mx);
     // P is rounded to the query's type for the second product (the sum l is not): half a step, 2^-8 (bf16) or 2^-11 (fp16)
     // of each weight, of both signs -- less in their sum than the rounding of the output itself
     u32x4 pf[BN / 16];
@@ -568,6 +561,14 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
 #pragma unroll
         for (int tb = 0; tb < NB; ++tb) nxt[tb] = Mma32<T>::run(w.k_frag(k_tile(buf ^ 1), ks, tb), w.qf[ks], nxt[tb]);
         weights(E * ks / KS & ~1, E * (ks + 1) / KS & ~1);
+        // the next requests, one at a time under the MFMAs: V of t + 1 over V of t - 1, then K of t + 2 over K of t (past the
+        // end of the range the last key's, which nobody reads: a branch here would cut the block that the compiler schedules)
+        if (ks < KS / 2) {
+          if (ks % kEvery == 0) request_one(false, buf ^ 1, ks / kEvery);
+        } else {
+          if (ks == KS / 2) rows_of(t + 2, entry);
+          if (ks % kEvery == 0) request_one(true, buf, (ks - KS / 2) / kEvery);
+        }
       }
       // pinned here: left to itself the compiler moves the weights behind the branches of finish_scores, next to their use
 #pragma unroll
@@ -579,7 +580,7 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
       weights(0, E);
       w.l += sum0 + sum1;
     }
-    mx = -INFINITY;
+    float mx = -INFINITY;
 #pragma unroll
     for (int st = 0; st < BN / 16; ++st)
 #pragma unroll
@@ -592,9 +593,11 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
           for (int e = E * at / N; e < E * (at + 1) / N; ++e) mx = fmaxf(mx, nxt[e / 16][e % 16]);
         }
       }
-    if constexpr (FP8 && NEXT) {
+    if constexpr (NEXT) {
+      w.move_reference(mx);                // (before the barrier, where the wave waits anyway)
       deposit(false, buf ^ 1);
-      if (t + 2 < t_last) deposit(true, buf);
+      deposit(true, buf);
+      entry = page_entry(t + 3);
     }
   };
 
@@ -628,17 +631,18 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
       float mx = -INFINITY;
 #pragma unroll
       for (int e = 0; e < E; ++e) mx = fmaxf(mx, s0[e / 16][e % 16]);
+      w.move_reference(mx);
       if (t_first + 1 < t_last) deposit(true, 1);
       int t = t_first;
       for (; t + 2 < t_last; t += 2) {       // two tiles a turn: the two sets of scores change places without copies
-        step(t, entry, mx, s0, s1, std::true_type{});
-        step(t + 1, entry, mx, s1, s0, std::true_type{});
+        step(t, entry, s0, s1, std::true_type{});
+        step(t + 1, entry, s1, s0, std::true_type{});
       }
       if (t + 1 < t_last) {
-        step(t, entry, mx, s0, s1, std::true_type{});
-        step(t + 1, entry, mx, s1, s0, std::false_type{});
+        step(t, entry, s0, s1, std::true_type{});
+        step(t + 1, entry, s1, s0, std::false_type{});
       } else {
-        step(t, entry, mx, s0, s1, std::false_type{});
+        step(t, entry, s0, s1, std::false_type{});
       }
     } else {
       if (t_first + 1 < t_last) deposit(true, 1);
@@ -646,9 +650,12 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
         const int buf = (t - t_first) & 1;
         publish();
         if (t + 1 >= t_last) continue;
-        fetch_next(t, buf, entry);
+        request(false, buf ^ 1);
+        rows_of(t + 2, entry);
+        entry = page_entry(t + 3);
+        request(true, buf);
         deposit(false, buf ^ 1);
-        if (t + 2 < t_last) deposit(true, buf);
+        deposit(true, buf);
       }
     }
   };

@@ -86,9 +86,15 @@ __device__ __forceinline__ float half_sum(float x) {
 // 16 bytes per lane from global memory to lds_base + 16 * lane.  Inline assembly, so that the compiler does not put a wait
 // for it in front of the LDS reads of the other buffer; the kernel waits itself (vmcnt(0)) before the barrier that
 // publishes the tile.  The instruction has no register output.
+// STREAM: past the caches, for rows that are read once.
+template <bool STREAM>
 __device__ __forceinline__ void load_to_lds_b128(const void* src, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src)
-               : "memory", "m0");
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(lds_base), "v"(src)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_base), "v"(src)
+                 : "memory", "m0");
 }
 
 __device__ __forceinline__ u32x4 lds_read_b128(const char* p) { return *(const u32x4*)p; }
@@ -508,7 +514,7 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
     if constexpr (FP8)
       (is_k ? f8k : f8v)[i] = *(const u32x4*)src;
     else
-      load_to_lds_b128(src, __builtin_amdgcn_readfirstlane(lds0 + (2 * buf + (is_k ? 0 : 1)) * kTileB + (i * NW + wave) * 1024));
+      load_to_lds_b128<false>(src, __builtin_amdgcn_readfirstlane(lds0 + (2 * buf + (is_k ? 0 : 1)) * kTileB + (i * NW + wave) * 1024));
   };
   auto request = [&](bool is_k, int buf) {
 #pragma unroll
@@ -725,7 +731,7 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
       if constexpr (FP8)
         (is_k ? f8k : f8v)[i] = load_stream_b128(src);
       else
-        load_to_lds_b128(src, __builtin_amdgcn_readfirstlane(lds0 + (is_k ? 0 : kTileB) + i * 1024));
+        load_to_lds_b128<true>(src, __builtin_amdgcn_readfirstlane(lds0 + (is_k ? 0 : kTileB) + i * 1024));
     }
   };
   auto deposit = [&](bool is_k) {

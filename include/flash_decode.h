@@ -613,7 +613,8 @@ FD_API int fd_pages_copy(void* stream, const fd_page_pool* pool, const int32_t* 
 
 /* Gives row b the pages that kv_lens[b] + new_tokens[b] tokens need (new_tokens NULL: `uniform` for every row).  ok[b]: 1, or
  * 0 where the table is too narrow or the pool has run out by then -- such a row keeps what it had.  Rows are served in
- * order, and a row that gets nothing still counts against the rows behind it.  batch <= 4096. */
+ * order, and a row that gets nothing still counts against the rows behind it.  batch <= 4096, and at most 2^20 new pages a
+ * row (a row that wants more is refused). */
 FD_API int fd_pages_reserve(void* stream, const fd_page_tables* tables, int32_t num_pages, int32_t page_size,
                             const int32_t* new_tokens, int32_t uniform, int32_t* ok);
 

@@ -108,7 +108,7 @@ def test_prefill_plan(fd):
     assert splits(16384, 1, 16384, paged=False) == 1 and splits(2048, 4, 32768) == 1
     assert splits(1, 1, 64) == 1 and splits(1, 1, 16384) > 8
     assert 1 < splits(256, 1, 16384) < splits(40, 1, 16384) <= 64
-    assert splits(1, 1, 16384, max_kv_len=200) == 1
+    assert splits(1, 1, 16384, max_kv_len=200) == 2 and splits(1, 1, 16384, max_kv_len=100) == 1
     assert splits(77, 1, 77, paged=False) == 1
 
 

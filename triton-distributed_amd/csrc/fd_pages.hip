@@ -129,6 +129,9 @@ constexpr int64_t kCopyGrid = 4096;   // workgroups that walk a list: 16 per CU
 // ---------------------------------------------------------------- reserve
 
 constexpr int kMaxReserveBatch = 4096;
+constexpr int kMaxReservePages = 1 << 20;     // of a row and call: 1024 rows' wants fit 32 bits ...
+constexpr int kWantedEnough = (1 << 30) - 1;  // ... and sums of more than any pool holds stop here
+constexpr int kNothingMissing = 0x7fffffff;
 
 __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const PageTables t, int num_pages, int P,
                                                                        const int32_t* __restrict__ new_tokens, int uniform,
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const Pa
     const int len = max(t.kv_lens[b], 0);
     const int64_t grown = (int64_t)len + max(new_tokens ? new_tokens[b] : uniform, 0);
     const int64_t last = (grown + P - 1) / P;
-    int missing = -1, first = 0;              // -1: the table has no room
+    int missing = -1, first = 0;              // -1: refused, the table has no room
     if (last <= t.width) {
       first = (int)(((int64_t)len + P - 1) / P);
       int have = 0;
@@ -150,7 +153,8 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const Pa
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) have += __shfl_xor(have, off);
       missing = max((int)last - first - have, 0);
-      first += have;
+      first = missing > 0 ? first + have : kNothingMissing;
+      if (missing > kMaxReservePages) missing = -1;
     }
     if (lane == 0) {
       s_end[b] = missing;
@@ -165,10 +169,10 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const Pa
     int total;
     const int incl = block_scan(max(need, 0), s_wave, &total);
     if (b < t.batch) {
-      s_end[b] = wanted + incl;
+      s_end[b] = min(wanted + incl, kWantedEnough);
       if (need < 0) s_at[b] = -1;
     }
-    wanted += total;
+    wanted = min(wanted + total, kWantedEnough);
   }
   __syncthreads();
   // how many of them the pool can give is known only when the scan has run; the pages are noted as they are found and a
@@ -186,10 +190,8 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const Pa
     t.bt[lo * t.sbt + s_at[lo] + (rank - before)] = page;
     t.refs[page] = 1;
   });
-  for (int b = threadIdx.x; b < t.batch; b += kScanThreads) {
-    const int need = s_end[b] - (b ? s_end[b - 1] : 0);
-    ok[b] = s_at[b] >= 0 && (need == 0 || s_end[b] <= found) ? 1 : 0;
-  }
+  for (int b = threadIdx.x; b < t.batch; b += kScanThreads)
+    ok[b] = s_at[b] == kNothingMissing || (s_at[b] >= 0 && s_end[b] <= found) ? 1 : 0;
 }
 
 // ---------------------------------------------------------------- fork

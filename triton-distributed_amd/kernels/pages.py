@@ -98,7 +98,7 @@ def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, tor
     """Gives every row the pages that its next ``new_tokens`` tokens need (an int for all rows, or int32 ``[B]``), so that
     the append that follows has somewhere to write.  Returns int32 ``[B]``: 1, or 0 where the table is too narrow or the
     pool has run out -- that row keeps what it had.  Rows are served in order; a row that gets nothing still counts against
-    the rows behind it.  At most 4096 rows."""
+    the rows behind it.  At most 4096 rows, and 2^20 new pages a row."""
     each = new_tokens if isinstance(new_tokens, torch.Tensor) else None
     batch = block_table.shape[0]
     _, t = _checked("paged_kv_reserve", (), (block_table, kv_lens, page_refs),

@@ -259,8 +259,8 @@ struct PrefillWave {
   f32x16 o[MB];
   float m, l;
 
-  // row0: first of the wave's rows; tok0: where in a tile its keys begin
-  __device__ __forceinline__ PrefillWave(const PrefillArgs& args, const PrefillItem& item, int row0, int tok0)
+  // row0: first of the wave's rows
+  __device__ __forceinline__ PrefillWave(const PrefillArgs& args, const PrefillItem& item, int row0)
       : a(args), it(item), lane(threadIdx.x & 63), half(lane >> 5), l32(lane & 31) {
     const int rows = it.n_q * a.G;
     const int row = min(row0 + l32, rows - 1);   // rows past the end repeat the last one and are not stored
@@ -488,7 +488,7 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
   static_assert(4 * kTileB <= kPrefillLds, "[2][K tile, V tile]");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r0 = it.j * BM, rows = it.n_q * a.G;
-  W w(a, it, r0 + wave * 32, 0);
+  W w(a, it, r0 + wave * 32);
   const int lane = w.lane;
   const int all_tiles = (max(it.limit_of(a, min(r0 + BM - 1, rows - 1)), 0) + BN - 1) / BN;
   const int per_split = max((all_tiles + it.splits - 1) / it.splits, it.min_tiles);
@@ -534,10 +534,10 @@ __device__ __forceinline__ void fd_row_tile(const PrefillArgs& a, const PrefillI
     __syncthreads();
   };
 
-  // One tile of the pipelined walk.  On entry `cur` holds tile t's finished scores, which the reference point
-  // has followed, pr the pool rows of tile t + 1, whose K is on its way, like V of tile t.  The scores of tile t + 1 are computed while the
-  // weights of tile t are (one MFMA and a few weights at a time: the matrix pipe works on one while the vector pipe does
-  // the others), and their maximum while V of tile t is multiplied.
+  // One tile of the pipelined walk.  On entry `cur` holds tile t's finished scores, which the reference point has followed,
+  // pr the pool rows of tile t + 1, whose K is on its way, like V of tile t.  The scores of tile t + 1 are computed while
+  // the weights of tile t are (one MFMA and a few weights at a time: the matrix pipe works on one while the vector pipe
+  // does the others), and their maximum while V of tile t is multiplied.
   constexpr int kEvery = KS / 2 / kLoads;  // k steps between two requests
   static_assert(KS == 2 * kEvery * kLoads, "the requests fit under the scores");
   constexpr int E = 16 * NB;               // scores of a lane
@@ -706,7 +706,7 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
   static_assert(2 * NW * kTileB <= kPrefillLds && (NW - 1) * kState * 4 <= kPrefillLds, "[NW][K tile, V tile]; the states");
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r0 = it.j * 32, rows = it.n_q * a.G;
-  W w(a, it, r0, 0);
+  W w(a, it, r0);
   const int lane = w.lane;
   const int hi_all = max(it.limit_of(a, min(r0 + 31, rows - 1)), 0);
   const int all_tiles = (hi_all + kUnit - 1) / kUnit;

@@ -5,8 +5,8 @@
 // the sequence's own keys behind them.  A wave has a row: its lanes take one LSE each, and 64 / (D / 4) groups of lanes, 128
 // bits a lane, share the partials among them.  The first of those are requested together with the LSEs -- an empty range's
 // partial may hold anything, its weight of 0 is never multiplied.  Bound: a launch and a dependent round trip or two where
-// there are few rows (4.6 us: 1280 rows of 8 partials), the partials' bytes else (6.5 us: 2048 rows of 17, 18 MB; 9.5 with D / 4 lanes a row and the
-// partials requested behind the LSEs).
+// there are few rows (4.6 us: 1280 rows of 8 partials), the partials' bytes else (6.5 us: 2048 rows of 17, 18 MB; 9.5 us with
+// D / 4 lanes a row and the partials requested behind the LSEs).
 #include "fd_prefill.h"
 
 namespace {

@@ -717,11 +717,11 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
   char* v_tile = k_tile + kTileB;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 2 * kTileB;
 
-  // ---- loads of a block: 16-byte chunk n = 64 i + lane.  fp8: into registers, `f8`
+  // ---- loads of a block: 16-byte chunk n = 64 i + lane
   auto page_entry = [&](int t0) { return it.page_entry(a, t0 + (lane & 31)); };
-  using Raw = u32x4[FP8 ? 2 * kLoads : 1];
-  auto request = [&](bool is_k, int row, Raw& f8) {
-    if (!FP8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was read of the block before has arrived
+  u32x4 f8k[FP8 ? kLoads : 1], f8v[FP8 ? kLoads : 1];
+  auto request = [&](bool is_k, int row) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // what was read of the block before has arrived
 #pragma unroll (kLoads > 8 ? 4 : kLoads)
     for (int i = 0; i < kLoads; ++i) {
       const int n = i * 64 + lane;
@@ -729,70 +729,47 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
       const char* src = (is_k ? w.kb : w.vb) + (uint64_t)(uint32_t)__shfl(row, r) * (is_k ? w.sk_b : w.sv_b)
                         + (W::source_chunk(is_k, r, ch) << 4);
       if constexpr (FP8)
-        f8[is_k ? i : kLoads + i] = load_stream_b128(src);
+        (is_k ? f8k : f8v)[i] = load_stream_b128(src);
       else
         load_to_lds_b128<true>(src, __builtin_amdgcn_readfirstlane(lds0 + (is_k ? 0 : kTileB) + i * 1024));
     }
   };
-  auto deposit = [&](Raw& f8) {
+  auto deposit = [&](bool is_k) {
     if constexpr (FP8) {
 #pragma unroll
-      for (int i = 0; i < 2 * kLoads; ++i) {
-        const int n = i % kLoads * 64 + lane;
-        W::deposit(i < kLoads, i < kLoads ? k_tile : v_tile, n / W::kInChunks, n % W::kInChunks, f8[i]);
+      for (int i = 0; i < kLoads; ++i) {
+        const int n = i * 64 + lane;
+        W::deposit(is_k, is_k ? k_tile : v_tile, n / W::kInChunks, n % W::kInChunks, (is_k ? f8k : f8v)[i]);
       }
-      wave_lds_fence();
     }
   };
-  // No barrier.  16-bit caches: one block deep per wave, K of the next block is requested when this one's scores are done, V
-  // when its product is; the waves of two workgroups cover each other's waits.  fp8, where a block is half the bytes: two
-  // blocks deep in registers, a block is requested as soon as the one two before it is in LDS.
+  // One block deep per wave and no barrier: K of the next block is requested when this one's scores are done, V when its
+  // product is; the waves of two workgroups cover each other's waits.
   auto walk = [&](auto careful_tag) {
     constexpr bool CAREFUL = decltype(careful_tag)::value;
-    constexpr int kStep = 32 * NW;
     w.start();
+    if (wave >= NW || lo + 32 * wave >= hi) return;
     int t0 = lo + 32 * wave;
-    if (wave >= NW || t0 >= hi) return;
-    auto pool_row = [&](int t, int entry) { return it.pool_row(a, t + (lane & 31), entry); };
-    if constexpr (FP8) {
-      Raw raw0, raw1;
-      int entry = page_entry(t0), ahead = page_entry(t0 + kStep);
-      auto request_both = [&](int t, Raw& f8) {   // (past the end: the last key's)
-        const int row = pool_row(t, entry);
-        request(true, row, f8);
-        request(false, row, f8);
-        entry = ahead;
-        ahead = page_entry(t + 2 * kStep);
-      };
-      auto block = [&](int t, Raw& f8) {
-        deposit(f8);
-        request_both(t + 2 * kStep, f8);
-        w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t, [] {});
-      };
-      request_both(t0, raw0);
-      request_both(t0 + kStep, raw1);
-      for (; t0 + kStep < hi; t0 += 2 * kStep) {
-        block(t0, raw0);
-        block(t0 + kStep, raw1);
-      }
-      if (t0 < hi) block(t0, raw0);
-    } else {
-      Raw none;
-      int row = pool_row(t0, page_entry(t0));
-      request(true, row, none);
-      request(false, row, none);
-      for (; t0 < hi; t0 += kStep) {
-        const int next = t0 + kStep;
+    int row = it.pool_row(a, t0 + (lane & 31), page_entry(t0));
+    request(true, row);
+    request(false, row);
+    for (; t0 < hi; t0 += 32 * NW) {
+      const int next = t0 + 32 * NW;
+      if constexpr (FP8) {
+        deposit(true);
+        deposit(false);
+        wave_lds_fence();
+      } else {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const int entry = next < hi ? page_entry(next) : 0;
-        w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t0, [&] {
-          if (next < hi) {
-            row = pool_row(next, entry);
-            request(true, row, none);
-          }
-        });
-        if (next < hi) request(false, row, none);
       }
+      const int entry = next < hi ? page_entry(next) : 0;
+      w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t0, [&] {
+        if (next < hi) {
+          row = it.pool_row(a, next + (lane & 31), entry);
+          request(true, row);
+        }
+      });
+      if (next < hi) request(false, row);
     }
   };
   walk(std::false_type{});

@@ -153,6 +153,20 @@ __device__ __forceinline__ int fd_tiles_before(int keys, int tiles, int n, int* 
   return before;
 }
 
+// The lane whose `keys` (at most `top`) are the rank-th largest of the wave's, equal ones in the order of their lanes: the
+// value bit by bit from above, then the lane among those that hold it.
+__device__ __forceinline__ int fd_lane_of_rank(int keys, int rank, int top) {
+  int value = 0;
+  for (int bit = 31 - __builtin_clz(top | 1); bit >= 0; --bit) {
+    const int with = value | 1 << bit;
+    if (__popcll(__ballot(keys >= with)) > rank) value = with;
+  }
+  const uint64_t equal = __ballot(keys == value);
+  const int at = rank - __popcll(__ballot(keys > value));
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(equal >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)equal, 0));
+  return __builtin_ctzll(__ballot(keys == value && before == at));
+}
+
 // The unit of this workgroup: KV head fastest (the eight XCDs take neighbouring workgroups in turn, so with eight KV heads
 // each XCD's L2 holds one head's keys), then the key range, then the row tile.  own: one of a shared-prefix step's sequences
 // with its own keys (tiles of 32 rows).  Those units, which are bound by memory, and the groups', which are bound by the
@@ -189,9 +203,7 @@ __device__ __forceinline__ bool fd_find_item(const PrefillArgs& a, int bm, Prefi
     if (place >= a.total_q) return false;
     const int b0 = place & ~63, n = min(64, a.total_q - b0);
     const int keys = lane < n ? min(max(a.own_lens[b0 + lane], 0), a.own_max_pages * a.P) : -1;
-    int total;
-    const int rank = fd_tiles_before(keys, 1, n, &total);
-    const int w = __builtin_ctzll(__ballot(lane < n && rank == place - b0));
+    const int w = fd_lane_of_rank(keys, place - b0, a.own_max_pages * a.P);
     it.q_start = b0 + w;
     it.n_k = __builtin_amdgcn_readlane(keys, w);
     it.n_q = 1;
@@ -717,11 +729,11 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
   char* v_tile = k_tile + kTileB;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + wave * 2 * kTileB;
 
-  // ---- loads of a block: 16-byte chunk n = 64 i + lane
+  // ---- loads of a block: 16-byte chunk n = 64 i + lane.  fp8: into registers, `f8`
   auto page_entry = [&](int t0) { return it.page_entry(a, t0 + (lane & 31)); };
-  u32x4 f8k[FP8 ? kLoads : 1], f8v[FP8 ? kLoads : 1];
-  auto request = [&](bool is_k, int row) {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    // what was read of the block before has arrived
+  using Raw = u32x4[FP8 ? 2 * kLoads : 1];
+  auto request = [&](bool is_k, int row, Raw& f8) {
+    if (!FP8) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was read of the block before has arrived
 #pragma unroll (kLoads > 8 ? 4 : kLoads)
     for (int i = 0; i < kLoads; ++i) {
       const int n = i * 64 + lane;
@@ -729,61 +741,88 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
       const char* src = (is_k ? w.kb : w.vb) + (uint64_t)(uint32_t)__shfl(row, r) * (is_k ? w.sk_b : w.sv_b)
                         + (W::source_chunk(is_k, r, ch) << 4);
       if constexpr (FP8)
-        (is_k ? f8k : f8v)[i] = load_stream_b128(src);
+        f8[is_k ? i : kLoads + i] = load_stream_b128(src);
       else
         load_to_lds_b128<true>(src, __builtin_amdgcn_readfirstlane(lds0 + (is_k ? 0 : kTileB) + i * 1024));
     }
   };
-  auto deposit = [&](bool is_k) {
-    if constexpr (FP8) {
+  auto deposit = [&](Raw& f8) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int n = i * 64 + lane;
-        W::deposit(is_k, is_k ? k_tile : v_tile, n / W::kInChunks, n % W::kInChunks, (is_k ? f8k : f8v)[i]);
-      }
+    for (int i = 0; i < 2 * kLoads; ++i) {
+      const int n = i % kLoads * 64 + lane;
+      W::deposit(i < kLoads, i < kLoads ? k_tile : v_tile, n / W::kInChunks, n % W::kInChunks, f8[i]);
     }
+    wave_lds_fence();
   };
-  // One block deep per wave and no barrier: K of the next block is requested when this one's scores are done, V when its
-  // product is; the waves of two workgroups cover each other's waits.
+  // No barrier.  16-bit caches: one block deep per wave, K of the next block is requested when this one's scores are done, V
+  // when its product is; the waves of two workgroups cover each other's waits.  fp8: kDeep blocks in registers, a block is
+  // requested as soon as the one kDeep before it is in LDS (own keys of 128 sequences: two deep is level with one, and one
+  // spills nothing).  Page entries are read a block ahead and before that block's requests: loads return in order, and the
+  // wait for an entry is one for what came before it.
   auto walk = [&](auto careful_tag) {
     constexpr bool CAREFUL = decltype(careful_tag)::value;
+    constexpr int kStep = 32 * NW;
     w.start();
-    if (wave >= NW || lo + 32 * wave >= hi) return;
     int t0 = lo + 32 * wave;
-    int row = it.pool_row(a, t0 + (lane & 31), page_entry(t0));
-    request(true, row);
-    request(false, row);
-    for (; t0 < hi; t0 += 32 * NW) {
-      const int next = t0 + 32 * NW;
-      if constexpr (FP8) {
-        deposit(true);
-        deposit(false);
-        wave_lds_fence();
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      const int entry = next < hi ? page_entry(next) : 0;
-      w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t0, [&] {
-        if (next < hi) {
-          row = it.pool_row(a, next + (lane & 31), entry);
-          request(true, row);
+    if (wave >= NW || t0 >= hi) return;
+    int entry = page_entry(t0), ahead = page_entry(t0 + kStep);
+    auto next_row = [&](int t) {                // the lane's row of block t (past the end: the last key's)
+      const int row = it.pool_row(a, t + (lane & 31), entry);
+      entry = ahead;
+      ahead = page_entry(t + 2 * kStep);
+      return row;
+    };
+    if constexpr (FP8) {
+      constexpr int kDeep = 1;
+      Raw raw[kDeep];
+      auto request_both = [&](int t, Raw& f8) {
+        const int row = next_row(t);
+        request(true, row, f8);
+        request(false, row, f8);
+      };
+#pragma unroll
+      for (int d = 0; d < kDeep; ++d) request_both(t0 + d * kStep, raw[d]);
+      for (; t0 < hi; t0 += kDeep * kStep) {
+#pragma unroll
+        for (int d = 0; d < kDeep; ++d) {       // (this form also keeps head dim 256 from spilling: 161 -> 92 us a step of
+          const int t = t0 + d * kStep;         // eight sequences of 8000 tokens)
+          if (t >= hi) break;
+          deposit(raw[d]);
+          request_both(t + kDeep * kStep, raw[d]);
+          w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t, [] {});
         }
-      });
-      if (next < hi) request(false, row);
+      }
+    } else {
+      Raw none;
+      int row = next_row(t0);
+      request(true, row, none);
+      request(false, row, none);
+      for (; t0 < hi; t0 += kStep) {
+        const int next = t0 + kStep;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        w.template plain_tile<1, CAREFUL>(k_tile, v_tile, t0, [&] {
+          if (next < hi) {
+            row = next_row(next);
+            request(true, row, none);
+          }
+        });
+        if (next < hi) request(false, row, none);
+      }
     }
   };
   walk(std::false_type{});
   if (w.not_finite()) walk(std::true_type{});
   w.l = half_sum(w.l);
-  // ---- join the waves' states in wave 0
+  // ---- join the states of the waves that had keys in wave 0
   float* st = (float*)smem;
   __syncthreads();
-  if (wave > 0 && wave < NW) {
+  if (wave > 0 && wave < NW && lo + 32 * wave < hi) {
     float* mine = st + (wave - 1) * kState;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mine[(mb * 16 + i) * 64 + lane] = w.o[mb][i];
+      for (int i = 0; i < 4; ++i)
+        *(f32x4*)(mine + ((mb * 4 + i) * 64 + lane) * 4) = f32x4{w.o[mb][4 * i], w.o[mb][4 * i + 1], w.o[mb][4 * i + 2], w.o[mb][4 * i + 3]};
     if (w.half == 0) {
       mine[D * 32 + w.l32] = w.m;
       mine[D * 32 + 32 + w.l32] = w.l;
@@ -791,26 +830,27 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
   }
   __syncthreads();
   if (wave > 0) return;
-  float top = w.m, f[NW];
-#pragma unroll
-  for (int k = 1; k < NW; ++k) top = fmaxf(top, st[(k - 1) * kState + D * 32 + w.l32]);
-  f[0] = fd_exp2(w.m - top);
-  w.l *= f[0];
-#pragma unroll
-  for (int k = 1; k < NW; ++k) {
-    f[k] = fd_exp2(st[(k - 1) * kState + D * 32 + w.l32] - top);
-    w.l += f[k] * st[(k - 1) * kState + D * 32 + 32 + w.l32];
-  }
+  const int others = min(NW, (hi - lo + 31) / 32) - 1;   // waves 1 .. others had keys
+  float top = w.m;
+  for (int k = 0; k < others; ++k) top = fmaxf(top, st[k * kState + D * 32 + w.l32]);
+  const float own = fd_exp2(w.m - top);
   w.m = top;
+  w.l *= own;
 #pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
+  for (int mb = 0; mb < MB; ++mb) w.o[mb] *= own;
+  for (int k = 0; k < others; ++k) {
+    const float* his = st + k * kState;
+    const float f = fd_exp2(his[D * 32 + w.l32] - top);
+    w.l += f * his[D * 32 + 32 + w.l32];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float x = w.o[mb][i] * f[0];
+    for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int k = 1; k < NW; ++k) x += f[k] * st[(k - 1) * kState + (mb * 16 + i) * 64 + lane];
-      w.o[mb][i] = x;
-    }
+      for (int i = 0; i < 4; ++i) {
+        const f32x4 x = *(const f32x4*)(his + ((mb * 4 + i) * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.o[mb][4 * i + e] += f * x[e];
+      }
+  }
   w.store();
 }
 

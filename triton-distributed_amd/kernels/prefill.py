@@ -142,6 +142,7 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     many, up to 64.
     """
     _check_no_grad("gqa_fwd_batch_prefill", q, k, v)
+    scale, soft_cap, causal = float(scale), float(soft_cap or 0.0), bool(causal)   # (values: a tensor could change under the key)
     key = (_sig(q), _sig(k), _sig(v), _sig(cu_seqlens_q), _sig(kv_lens), _sig(block_table), _sig(cu_seqlens_k), _sig(q_lens),
            _sig(output), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, causal, max_kv_len, kv_split)
     cached = _PREFILL_CACHE.get(key)
@@ -258,6 +259,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     queries with a cache of the same type or fp8-e4m3.  ``max_kv_len`` / ``max_prefix_len``: host-side hints.
     """
     _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache)
+    scale, soft_cap = float(scale), float(soft_cap or 0.0)
     # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
     hints = (-(-max_kv_len // 1024) * 1024 if max_kv_len else 0, -(-max_prefix_len // 1024) * 1024 if max_prefix_len else 0)
     key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(kv_lens), _sig(block_table), _sig(prefix_lens), _sig(prefix_table),

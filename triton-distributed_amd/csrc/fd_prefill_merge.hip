@@ -4,7 +4,8 @@
 // M = max_s LSE_s, LSE = M + log sum_s w_s.  In a shared-prefix step the ranges of the group's prefix come first and those of
 // the sequence's own keys behind them.  A wave has a row: its lanes take one LSE each, and 64 / (D / 4) groups of lanes, 128
 // bits a lane, share the partials among them.  The first of those are requested together with the LSEs -- an empty range's
-// partial may hold anything, its weight of 0 is never multiplied.  Bound: a launch and a dependent round trip or two where
+// partial may hold anything, its weight of 0 is never multiplied.  A NaN LSE -- a row that met a NaN -- makes the row NaN, in
+// out and LSE, as it does where one range is stored without a merge.  Bound: a launch and a dependent round trip or two where
 // there are few rows (4.6 us: 1280 rows of 8 partials), the partials' bytes else (6.5 us: 2048 rows of 17, 18 MB; 9.5 us with
 // D / 4 lanes a row and the partials requested behind the LSEs).
 #include "fd_prefill.h"
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(256) fd_prefill_merge_kernel(const PrefillArgs
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
     top = fmaxf(top, M);
-    if (top == -INFINITY) continue;
+    if (top == -INFINITY && !__any(mine != mine)) continue;   // nothing seen so far (a NaN LSE, which fmaxf drops, is not that)
     const float keep = __expf(M - top);        // 0 in the first pass that counts
     acc *= keep;
     M = top;

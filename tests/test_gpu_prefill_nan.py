@@ -73,3 +73,23 @@ def test_a_nan_query_of_a_shared_prefix_step(fd, Hq, Hkv, D, fp8):
         q.to(DEV), pg.k, pg.v, None, [1] * B, pg.lens[:B].to(DEV), pg.table[:B].to(DEV), pg.lens[B:].to(DEV),
         pg.table[B:].to(DEV), D ** -0.5, group_starts=starts(members).to(DEV), lse_out=lse, **pg.kw)
     check_rows(out, lse, ref, nan_rows, BF16, 500, pg.vmax)
+
+
+@pytest.mark.parametrize("cap", [0.0, 8.0])
+@pytest.mark.parametrize("tokens,kv_split", [(3, 1), (3, 4), (150, 1)])
+def test_a_nan_scale(fd, cap, tokens, kv_split):
+    """The softmax scale, and one KV head's scale of an fp8 cache; rows that see no key stay 0."""
+    g = torch.Generator().manual_seed(53)
+    Hq, Hkv, D = 8, 2, 128
+    ql, kl = [tokens, tokens], [200, tokens - 2]            # (the second sequence: two rows without a key)
+    pg = Paged(kl, Hkv, D, 16, BF16, fp8=True, seed=3)
+    q = torch.randn(2 * tokens, Hq, D, generator=g).to(BF16)
+    ref = oracle_prefill(q, pg.seq, ql, True, 0.09, cap)
+    sees = torch.isfinite(ref[1])
+    k_scale = pg.kw["k_scale"].clone()
+    k_scale[1] = math.nan
+    for scale, ks, nan_rows in ((math.nan, pg.kw["k_scale"], sees), (0.09, k_scale, sees & (torch.arange(Hq) >= 4))):
+        lse = torch.empty(2 * tokens, Hq, device=DEV)
+        out = fd.gqa_fwd_batch_prefill(q.to(DEV), pg.k, pg.v, starts(ql).to(DEV), pg.lens.to(DEV), pg.table.to(DEV), scale,
+                                       cap, lse_out=lse, kv_split=kv_split, k_scale=ks, v_scale=pg.kw["v_scale"])
+        check_rows(out, lse, ref, nan_rows, BF16, 200, pg.vmax)

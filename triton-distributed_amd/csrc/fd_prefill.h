@@ -452,8 +452,11 @@ struct PrefillWave {
   }
 
   // l: already summed over the wave halves
-  __device__ __forceinline__ void store() const {
+  __device__ __forceinline__ void store() {
     if (!real_row) return;
+    // a NaN scale: the lower bound of c dropped it (kept apart from the scores, it leaves rows that see nothing as they are)
+    const float scale = FP8 ? a.sm_scale * a.k_scale[it.kvh] : a.sm_scale;
+    if (scale != scale && my_limit > 0) l = scale;
     float inv = l != 0.f ? 1.0f / l : 0.f;
     const float lse = l != 0.f ? m * FD_LN2 + __logf(l) : -INFINITY;
     if (FP8) inv *= a.v_scale[it.kvh];

@@ -10,7 +10,8 @@ one between steps is here.  The state is three tensors on the GPU next to the po
 The pools are ``[pages, P, Hkv, D]``, or ``[layers, pages, P, Hkv, D]`` for all layers of a model at once (one table for
 all of them).  Every function changes these tensors in place, enqueues its kernels through the C ABI in
 ``include/flash_decode.h`` (``fd_pages_*``) on the current (or given) stream and reads nothing on the host.  A free page is
-handed out lowest id first, in the order of the requests.  Calls on one cache must follow each other on one stream.
+handed out lowest id first, in the order of the requests.  Calls on one cache must follow each other on one stream.  ``stream=``
+as in ``kernels/prefill.py``.
 """
 from __future__ import annotations
 
@@ -104,7 +105,7 @@ def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, tor
     _, t = _checked("paged_kv_reserve", (), (block_table, kv_lens, page_refs),
                     (("new_tokens", each, (batch,)), ("ok_out", ok_out, (batch,))))
     if ok_out is None:
-        ok_out = _new(batch, torch.int32, block_table.device, stream)
+        ok_out = _new(batch, torch.int32, block_table.device, stream, returned=True)
     _need(batch <= 4096, f"paged_kv_reserve: {batch} rows (at most 4096)")
     _need(each is not None or 0 <= new_tokens < 1 << 31, f"paged_kv_reserve: new_tokens {new_tokens}")
     if batch:
@@ -124,7 +125,7 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
     pool, t = _checked("paged_kv_fork", (k_cache, v_cache), (block_table, kv_lens, page_refs),
                        (("parents", parents, (n,)), ("children", children, (n,)), ("ok_out", ok_out, (n,))))
     if ok_out is None:
-        ok_out = _new(n, torch.int32, k_cache.device, stream)
+        ok_out = _new(n, torch.int32, k_cache.device, stream, returned=True)
     if n:
         lib = load_library()
         need = lib.fd_pages_workspace_bytes(pool.num_pages, n)
@@ -150,7 +151,7 @@ def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Opti
     row that holds pages.  Returns int32 ``[1]`` (on the device): ``n``, from where on the pool is free."""
     pool, t = _checked("paged_kv_compact", (k_cache, v_cache), (block_table, None, page_refs), (("live_out", live_out, (1,)),))
     if live_out is None:
-        live_out = _new(1, torch.int32, k_cache.device, stream)
+        live_out = _new(1, torch.int32, k_cache.device, stream, returned=True)
     lib = load_library()
     need = lib.fd_pages_workspace_bytes(pool.num_pages, 0)
     ws = _new(need, torch.uint8, k_cache.device, stream)

@@ -9,6 +9,9 @@ share a prefix.
 Every function enqueues hand-written HIP kernels through the C ABI in ``include/flash_decode.h`` (``fd_prefill``,
 ``fd_decode_shared``); nothing synchronises with the host, lengths are never read on it, and there is no CPU path.  Forward
 only: a query, key or value that requires a gradient is refused while autograd records.
+
+``stream=`` enqueues a call's kernels there instead of on the current stream.  The caller orders it behind what the arguments
+need and what uses the result behind it, and keeps the arguments alive; what the call allocates needs no ordering.
 """
 from __future__ import annotations
 
@@ -71,6 +74,7 @@ def _check_table(name, what, table, rows):
 
 def _launch(fn, device, stream, *args):
     """Calls the library on the tensors' device, whatever the current one is, and raises what it reports."""
+    _need(stream is None or stream.device == device, f"tensors on {device}, a stream of another device")
     if device.index == torch.cuda.current_device():
         rc = fn(stream_handle(stream, device.index), *args)
     else:
@@ -85,11 +89,15 @@ def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-def _new(shape, dtype, device, stream):
-    """A tensor that work on ``stream`` uses although it was allocated for the current one."""
-    t = torch.empty(shape, dtype=dtype, device=device)
-    if stream is not None:
-        t.record_stream(stream)
+def _new(shape, dtype, device, stream, returned=False):
+    """A new tensor for work on ``stream`` (None: the current one).  It comes from that stream's pool: a block of the current
+    stream's may still be in use by work that is queued there.  ``returned``: the caller may use it on the current stream."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if returned:
+        t.record_stream(torch.cuda.current_stream(device))
     return t
 
 
@@ -152,7 +160,7 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
             q_lens, output, lse_out, k_scale, v_scale, max_kv_len, kv_split))
     image, need = cached
     if output is None:
-        output = _new(q.shape, q.dtype, q.device, stream)
+        output = _new(q.shape, q.dtype, q.device, stream, returned=True)
     if image is None:      # no rows, or no sequence
         return output
     a = FdPrefillArgs.from_buffer_copy(image)
@@ -271,7 +279,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
             soft_cap, group_starts, output_combine, lse_out, k_scale, v_scale, hints))
     image, need = cached
     if output_combine is None:
-        output_combine = _new(q.shape, q.dtype, q.device, stream)
+        output_combine = _new(q.shape, q.dtype, q.device, stream, returned=True)
     if image is None:      # no sequence
         return output_combine
     a = FdSharedArgs.from_buffer_copy(image)

@@ -5,6 +5,7 @@ import torch
 
 from test_gpu_pages import Pair
 from test_gpu_prefill import BF16, DEV, Paged, check, oracle_prefill, oracle_shared, starts
+from test_gpu_serving import make_block, positions
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +64,30 @@ def test_pages(fd):
         want = t.m.fork([0, 0, 2, 5], [1, 3, 4, 6]), t.m.reserve([9] * 12), t.m.compact()
         assert (forked.tolist(), granted.tolist(), int(live)) == want
         t.same()
+
+
+def test_the_block_on_a_stream(fd):
+    """A prompt and a decode step through the block on another stream while the current one is busy."""
+    gen = torch.Generator().manual_seed(1)
+    B, hidden, Hq, Hkv, D, T = 2, 256, 8, 2, 128, 37
+    attn, tab = make_block(fd, hidden, Hq, Hkv, D, gen)
+    x = torch.randn(B, T + 1, hidden, generator=gen).to(BF16).to(DEV)
+    got = []
+    for on_side in (False, True):
+        cache = fd.layers.PagedKV_Cache(num_layers=1, batch_size=B, max_length=256, kv_heads=Hkv, head_dim=D, dtype=BF16,
+                                        page_size=16, seed=4)
+        pos = positions(cache, T, B), positions(cache, 1, B) + T
+        first, last = x[:, :T].contiguous(), x[:, T:].contiguous()
+        side = side_stream()
+        kw = {"stream": side} if on_side else {}
+        if on_side:
+            leave_writes_pending(B * T * (Hq + 2 * Hkv) * D * 2, B * T * Hq * D * 2, B * T * hidden * 2, B * 4, B * hidden * 2)
+        y = attn.prefill(first, pos[0], tab, cache, 0, **kw)
+        with torch.cuda.stream(kw.get("stream", torch.cuda.current_stream())):
+            cache.inc_offset(T)
+        z = attn.fwd(last, pos[1], tab, cache, 0, **kw)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        got.append((y, z, cache.k_cache, cache.v_cache))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)

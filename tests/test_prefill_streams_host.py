@@ -18,8 +18,10 @@ def test_memory_for_a_stream_comes_from_its_pool(fd, monkeypatch):
     @contextlib.contextmanager
     def enter(s):
         inside.append(s)
-        yield
-        inside.pop()
+        try:
+            yield
+        finally:
+            inside.pop()
 
     class Tensor(torch.Tensor):
         def record_stream(self, s):
@@ -45,3 +47,32 @@ def test_a_stream_of_another_device_is_refused(fd):
     pre = importlib.import_module(fd.__name__ + ".kernels.prefill")
     with pytest.raises(RuntimeError, match="another device"):
         pre._launch(lambda *a: 0, torch.device("cuda", 1), _Stream())
+
+
+def test_the_block_enters_the_stream_before_any_of_its_work(fd, monkeypatch):
+    """``prefill`` and ``fwd``: the first projection already runs on the given stream."""
+    inside = []
+
+    @contextlib.contextmanager
+    def enter(s):
+        inside.append(s)
+        try:
+            yield
+        finally:
+            inside.pop()
+
+    class Reached(Exception):
+        pass
+
+    def linear(*args):
+        seen.append(inside[-1] if inside else "current")
+        raise Reached
+
+    monkeypatch.setattr(torch.cuda, "stream", enter)
+    monkeypatch.setattr(torch.nn.functional, "linear", linear)
+    attn, side, seen = fd.layers.TP_Attn(), _Stream(), []
+    for method, n in ((attn.prefill, 3), (attn.fwd, 1)):
+        for kw in ({"stream": side}, {}):
+            with pytest.raises(Reached):
+                method(torch.zeros(2, n, 8), None, None, None, 0, **kw)
+    assert seen == [side, "current"] * 2

@@ -14,6 +14,7 @@ are other paths -- and anything else raises.
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -37,6 +38,20 @@ def _set_cos_sin_cache(inv_freq: torch.Tensor, max_length: int):
     t = torch.arange(max_length, device=inv_freq.device, dtype=inv_freq.dtype)
     freqs = torch.outer(t, inv_freq)
     return torch.cat((freqs.cos(), freqs.sin()), dim=-1).to(torch.float32).contiguous()
+
+
+def _on_stream(method):
+    """``method`` with ``stream=``: all of its work on that stream, projections included; the caller orders the stream behind
+    what the arguments need and what uses the result behind it."""
+    @functools.wraps(method)
+    def call(self, *args, stream=None, **kw):
+        if stream is None:
+            return method(self, *args, **kw)
+        with torch.cuda.stream(stream):
+            out = method(self, *args, **kw)
+        out.record_stream(torch.cuda.current_stream(out.device))
+        return out
+    return call
 
 
 class TP_Attn:
@@ -79,12 +94,14 @@ class TP_Attn:
         """The reference builds its all-gather / reduce-scatter GEMM contexts here (tp_attn.py:211-230); one GPU
         needs none."""
 
+    @_on_stream
     @torch.inference_mode()
     def fwd(self, x: torch.Tensor, position_ids: torch.Tensor, cos_sin_cache: torch.Tensor, kv_cache, layer_idx: int,
             **decode_kw):
         """x ``[B, 1, hidden]`` -> ``[B, 1, hidden]``; appends the token's K/V to ``kv_cache`` at its offsets.
         The caller advances the offsets afterwards (``kv_cache.inc_offset()``), as the reference's engine does
-        (models/engine.py:168)."""
+        (models/engine.py:168).  ``stream=``: the whole block runs there; other keywords go to
+        ``flash_attn_with_kvcache``."""
         bsz, q_len, _ = x.size()
         if q_len != 1:
             raise NotImplementedError("TP_Attn.fwd: decode step only (one new token per sequence)")
@@ -103,6 +120,7 @@ class TP_Attn:
                                       q_norm=q_norm, k_norm=k_norm, **decode_kw)
         return nn.functional.linear(out.view(bsz, q_len, -1), self.wo)
 
+    @_on_stream
     @torch.inference_mode()
     def prefill(self, x: torch.Tensor, position_ids: torch.Tensor, cos_sin_cache: torch.Tensor, kv_cache, layer_idx: int,
                 q_lens: Optional[torch.Tensor] = None, **prefill_kw):
@@ -111,7 +129,8 @@ class TP_Attn:
         included), then causal attention covers cache and chunk.  ``q_lens`` (int32 ``[B]``): a batch padded to T, only the
         first ``q_lens[b]`` tokens of sequence b are real; what the padding wrote behind a sequence's length is
         overwritten by its next tokens, and its rows of the result mean nothing.  The caller advances the offsets
-        (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  Keywords go to ``gqa_fwd_batch_prefill``."""
+        (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  ``stream=``: the whole block runs there; other keywords
+        go to ``gqa_fwd_batch_prefill``."""
         bsz, q_len, _ = x.size()
         if q_len == 0:
             return x.new_empty(bsz, 0, self.wo.shape[0])

@@ -91,3 +91,50 @@ def test_the_block_on_a_stream(fd):
         got.append((y, z, cache.k_cache, cache.v_cache))
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_the_cached_attention_call(fd, shared):
+    """Append, rotation and decode step in one call on another stream: grown lengths, rotated queries and results are its own."""
+    B, Hq, Hkv, D, P = 6, 8, 2, 128, 16
+    g = torch.Generator().manual_seed(5)
+    lens = torch.tensor([40, 300, 5, 77, 1, 160], dtype=torch.int32, device=DEV)
+    table = torch.randperm(B * 32, generator=g).int().view(B, 32).to(DEV)
+    q, k, v = (torch.randn(B, 1, h, D, generator=g).to(BF16).to(DEV) for h in (Hq, Hkv, Hkv))
+    pools = [torch.randn(B * 32 + 8, P, Hkv, D, generator=g).to(BF16).to(DEV) for _ in range(2)]
+    tab = fd.layers._set_cos_sin_cache((1.0 / 10000.0 ** (torch.arange(0, D, 2, dtype=torch.float32) / D)).to(DEV), 1024)
+    kw = dict(k=k, v=v, cache_seqlens=lens, block_table=table, cos_sin_cache=tab, position_ids=lens[:, None].long(),
+              return_softmax_lse=True)
+    if shared:
+        kw["shared_prefix"] = (torch.tensor([100], dtype=torch.int32, device=DEV),
+                               torch.arange(B * 32, B * 32 + 7, dtype=torch.int32, device=DEV).view(1, 7), None)
+    got = []
+    for on_side in (False, True, True):
+        kc, vc = (p.clone() for p in pools)
+        side = side_stream()
+        if on_side:
+            leave_writes_pending(B * 4, B * Hq * 4, B * Hq * D * 2, 1 << 20, 2 << 20)
+        out, lse = fd.flash_attn_with_kvcache(q, kc, vc, **kw, **({"stream": side} if on_side else {}))
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        got.append((out, lse, kc, vc))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fuse", [False, True])
+def test_decode_twins_on_a_stream(fd, fuse):
+    pg = Paged([1, 400, 77, 1030], 8, 128, 16, BF16, seed=4)
+    q = torch.randn(4, 32, 128, generator=torch.Generator().manual_seed(2)).to(BF16)
+    args = (q.to(DEV), pg.k, pg.v, None, [1] * 4, pg.lens.to(DEV), pg.table.to(DEV), 0.09)
+    want = oracle_prefill(q, pg.seq, [1] * 4, True, 0.09)
+    need = fd.workspace_bytes(args[0], pg.k, args[6])
+    for _ in range(3):
+        lse = torch.empty(4, 32, device=DEV)
+        side = side_stream()
+        leave_writes_pending(q.numel() * 2, need, 4 * 4096)
+        out = fd.gqa_fwd_batch_decode_aot(side, *args, lse_out=lse, fuse_combine=fuse)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        check(out, lse, *want, BF16, 1030, pg.vmax)

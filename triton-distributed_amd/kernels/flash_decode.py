@@ -102,13 +102,25 @@ def _require_cuda(*tensors):
             raise RuntimeError("flash-decode tensors must live on the GPU; this package has no CPU path")
 
 
+def _new(shape, dtype, device, stream, returned=False):
+    """A new tensor for work on ``stream`` (None: the current one).  It comes from that stream's pool: a block of the current
+    stream's may still be in use by work that is queued there.  ``returned``: the caller may use it on the current stream."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=device)
+    if returned:
+        t.record_stream(torch.cuda.current_stream(device))
+    return t
+
+
 def schedule_sequences(kv_lens: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """Kernel (3): int32 [B] sequence order, longest kv_len first, computed on the device."""
     _require_cuda(kv_lens)
     lib = load_library()
     assert kv_lens.dtype == torch.int32 and kv_lens.is_contiguous()
     if out is None:
-        out = torch.empty_like(kv_lens)
+        out = _new(kv_lens.shape, torch.int32, kv_lens.device, stream, returned=True)
     check(lib.fd_schedule(stream_handle(stream, kv_lens.device.index), kv_lens.data_ptr(), kv_lens.numel(),
                           out.data_ptr()))
     return out
@@ -255,7 +267,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
     if output_combine is None:
         if no_alloc:
             raise RuntimeError("no_alloc=True needs output_combine")
-        output_combine = torch.empty([batch, q_heads, out_cols], dtype=q.dtype, device=q.device)
+        output_combine = _new([batch, q_heads, out_cols], q.dtype, q.device, stream, returned=True)
     else:
         _require_cuda(output_combine)
     oc_st = output_combine.stride()
@@ -329,9 +341,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
                 and workspace.numel() * workspace.element_size() >= need):
             hold = workspace     # the caller's workspace is large enough: no allocation in the call
         else:
-            hold = torch.empty(need, dtype=torch.uint8, device=q.device)
-            if stream is not None:   # freed on return: keep the allocator from reusing it before `stream` is done
-                hold.record_stream(stream)
+            hold = _new(need, torch.uint8, q.device, stream)
         a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
         a.workspace, a.workspace_bytes = hold.data_ptr(), need
         a.out, a.block_table, a.kv_lens = output_combine.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr()
@@ -397,17 +407,13 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
                 and workspace.is_contiguous() and workspace.numel() >= n_o + n_l):
             hold = workspace
         else:
-            hold = torch.empty(n_o + n_l, dtype=torch.float32, device=q.device)
-            if stream is not None:
-                hold.record_stream(stream)
+            hold = _new(n_o + n_l, torch.float32, q.device, stream)
         mid_ptr = hold.data_ptr() if hold is not None else None
         lse_split_ptr = mid_ptr + 4 * n_o if hold is not None else None
         so_b, so_h, so_s = q_heads * num_splits * v_head_dim, num_splits * v_head_dim, v_head_dim
     want_items = (item_order is not None and num_splits > 1 and not fuse_combine) or plan.order_kind == FD_ORDER_ITEMS
     if plan.order_kind == FD_ORDER_SEQUENCES:
         seq_order = schedule_sequences(kv_lens, stream=stream)
-        if stream is not None:
-            seq_order.record_stream(stream)
     p = _make_params(q, k_cache, block_table, num_splits, soft_cap, plan.mid_dtype, out_dtype, k_scale, v_scale, path,
                      waves_per_block, seq_order_lens, plan.split_align, plan.split_adapt, 0, plan.max_kv_len, v_head_dim)
     if want_items:
@@ -415,9 +421,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
         # it) or computed here by one scheduling launch.  With the caller's exact split count the items are the
         # reference's ranges (every slot of the partial buffer is still written, empty ranges last).
         if item_order is None:
-            item_order = item_order_buffer(batch, num_splits, q.device)
-            if stream is not None:
-                item_order.record_stream(stream)
+            item_order = _new(2 * batch * num_splits, torch.int32, q.device, stream)
             check(lib.fd_schedule_items(hstream, kv_lens.data_ptr(), batch, item_order.data_ptr(), byref(p)))
         assert item_order.dtype == torch.int32 and item_order.is_contiguous()
         assert item_order.numel() >= 2 * batch * num_splits
@@ -435,7 +439,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
             oc_st[0], oc_st[1], seq_order.data_ptr() if seq_order is not None else None, mode,
             ex_out.data_ptr() if n_extra else None, ex_lse.data_ptr() if n_extra else None, n_extra, byref(p)))
         return output_combine
-    tickets = _tickets(q.device, hstream, batch * q_heads) if fuse_combine else None
+    tickets = _tickets(q.device, hstream, batch * q_heads, stream) if fuse_combine else None
     check(lib.fd_decode(
         hstream, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), mid_ptr, lse_split_ptr,
         output_combine.data_ptr(), lse_out.data_ptr() if lse_out is not None else None, float(scale),
@@ -478,7 +482,7 @@ class PreparedDecode:
             kw["schedule_items"] = True
         cols = v_cache.shape[-1] + (1 if variant == "intra_rank" else 0)
         if output_combine is None:
-            output_combine = torch.empty(q.shape[0], q.shape[1], cols, dtype=q.dtype, device=q.device)
+            output_combine = _new((q.shape[0], q.shape[1], cols), q.dtype, q.device, stream, returned=True)
         self._lib = load_library()
         self._stream = stream
         self._device = q.device.index
@@ -516,12 +520,13 @@ _PLAN_CACHE = {}   # fd_plan_decode results by problem shape
 _TICKETS = {}
 
 
-def _tickets(device, hstream, n):
+def _tickets(device, hstream, n, stream):
     key = (device.index, hstream)
     t = _TICKETS.get(key)
     if t is None or t.numel() < n:
-        t = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
-        _TICKETS[key] = t
+        t = _TICKETS[key] = _new(max(n, 4096), torch.int32, device, stream)
+        with torch.cuda.stream(stream):      # (None: the current one)
+            t.zero_()
     return t
 
 

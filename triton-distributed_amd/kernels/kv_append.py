@@ -14,6 +14,7 @@ Every function enqueues hand-written HIP kernels through the C ABI in
 """
 from __future__ import annotations
 
+import functools
 from ctypes import byref
 from typing import Optional, Tuple, Union
 
@@ -47,6 +48,23 @@ def _prep_struct(cos_sin, position_ids, head_dim, bsz, seq) -> FdQkPrep:
     return r
 
 
+def _on_stream(fn):
+    """``fn`` with ``stream=``: all of its work, and what it allocates, on that stream; the caller orders the stream behind
+    what the arguments need and what uses the result behind it."""
+    @functools.wraps(fn)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return fn(*args, **kw)
+        with torch.cuda.stream(stream):
+            out = fn(*args, **kw)
+        for t in out if isinstance(out, tuple) else (out,):
+            if t is not None:
+                t.record_stream(torch.cuda.current_stream(t.device))   # (the caller uses it there)
+        return out
+    return call
+
+
+@_on_stream
 def rope_kv_append(k_new: Optional[torch.Tensor], v_new: Optional[torch.Tensor], k_cache: Optional[torch.Tensor],
                    v_cache: Optional[torch.Tensor], block_table: Optional[torch.Tensor],
                    kv_lens: Optional[torch.Tensor], *, kv_lens_out: Optional[torch.Tensor] = None,
@@ -56,7 +74,7 @@ def rope_kv_append(k_new: Optional[torch.Tensor], v_new: Optional[torch.Tensor],
                    cos_sin: Optional[torch.Tensor] = None, position_ids: Optional[torch.Tensor] = None,
                    q: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None,
                    q_norm: Optional[Tuple[torch.Tensor, float]] = None,
-                   k_norm: Optional[Tuple[torch.Tensor, float]] = None, stream=None):
+                   k_norm: Optional[Tuple[torch.Tensor, float]] = None):
     """Appends ``k_new`` / ``v_new`` ``[B, T, Hkv, D]`` at positions ``kv_lens[b] .. +T-1`` of the paged pool.
 
     With ``cos_sin`` (fp32 ``[max_pos, D]``) and ``position_ids`` (``[B, T]`` int32/int64) K is rotated before it
@@ -140,7 +158,7 @@ def rope_kv_append(k_new: Optional[torch.Tensor], v_new: Optional[torch.Tensor],
     elif q is not None:
         raise RuntimeError("rope_kv_append: q is only processed together with cos_sin / position_ids or a norm")
     check(lib.fd_kv_append(
-        stream_handle(stream, src.device.index), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
+        stream_handle(None, src.device.index), _ptr(k_new), _ptr(v_new), _ptr(k_cache), _ptr(v_cache),
         _ptr(block_table), _ptr(kv_lens), _ptr(kv_lens_out), _ptr(seq_order_out), bsz, seq, *skn, *svn, *sk, *sv, sbt,
         byref(prep) if prep is not None else None, byref(p)))
     return q_out if q is not None else None
@@ -174,12 +192,13 @@ def _dense_block_table(device, n):
     return t
 
 
+@_on_stream
 def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None, rotary_sin=None,
                             cache_seqlens: Union[int, torch.Tensor, None] = None, cache_batch_idx=None,
                             cache_leftpad=None, block_table=None, softmax_scale=None, causal=False,
                             window_size=(-1, -1), softcap=0.0, rotary_interleaved=True, alibi_slopes=None,
                             num_splits=0, return_softmax_lse=False, *, cos_sin_cache=None, position_ids=None,
-                            k_scale=None, v_scale=None, kv_lens_out=None, q_norm=None, k_norm=None, stream=None,
+                            k_scale=None, v_scale=None, kv_lens_out=None, q_norm=None, k_norm=None,
                             shared_prefix=None, **decode_kw):
     """Decode-step drop-in for the flash-attn call of the reference's attention block (tp_attn.py:268-269).
 
@@ -254,13 +273,13 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
                                seq_order_out=order, item_order_out=items, item_plan=item_plan,
                                k_scale=k_scale, v_scale=v_scale,
                                cos_sin=cos_sin_cache, position_ids=position_ids, q=q if prep_q else None,
-                               q_norm=q_norm, k_norm=k_norm, stream=stream)
+                               q_norm=q_norm, k_norm=k_norm)
         if q_rot is None:
             q_rot = q
         kv_lens = kv_lens_out
     elif cos_sin_cache is not None or q_norm is not None:
         q_rot = rope_kv_append(None, None, None, None, None, None, cos_sin=cos_sin_cache, position_ids=position_ids,
-                               q=q, q_norm=q_norm, stream=stream)
+                               q=q, q_norm=q_norm)
 
     out = torch.empty_like(q)
     lse = torch.empty((bsz, q_heads), dtype=torch.float32, device=dev) if return_softmax_lse else None
@@ -269,12 +288,12 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         gqa_fwd_batch_decode_shared_prefix(q_rot[:, 0], k_cache, v_cache, None, None, kv_lens, block_table, prefix_lens,
                                            prefix_table, scale, softcap, group_starts=group_starts,
                                            output_combine=out[:, 0], lse_out=lse, k_scale=k_scale, v_scale=v_scale,
-                                           stream=stream, **decode_kw)
+                                           **decode_kw)
         return (out, lse.view(bsz, q_heads, 1)) if return_softmax_lse else out
     _decode(q_rot.view(bsz, q_heads, head_dim) if q_rot.is_contiguous() else q_rot[:, 0], k_cache, v_cache, None,
             kv_lens, block_table, scale, softcap, None, out.view(bsz, q_heads, head_dim),
             num_splits if num_splits > 0 else -1, with_lse_column=False, lse_out=lse, k_scale=k_scale, v_scale=v_scale,
-            stream=stream, **decode_kw)
+            **decode_kw)
     if return_softmax_lse:
         return out, lse.view(bsz, q_heads, 1)
     return out

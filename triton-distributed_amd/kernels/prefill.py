@@ -22,7 +22,7 @@ import torch
 
 from .._lib import (FD_COMBINE_SPLIT, FdParams, FdPrefillArgs, FdSharedArgs, check, fd_dtype_of, load_library,
                     stream_handle)
-from .flash_decode import _require_cuda
+from .flash_decode import _new, _require_cuda
 
 
 def _need(condition, message):
@@ -87,18 +87,6 @@ def _launch(fn, device, stream, *args):
 def _sig(t):
     """What the checks of an argument look at: a call whose arguments have all been seen before skips them."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
-
-
-def _new(shape, dtype, device, stream, returned=False):
-    """A new tensor for work on ``stream`` (None: the current one).  It comes from that stream's pool: a block of the current
-    stream's may still be in use by work that is queued there.  ``returned``: the caller may use it on the current stream."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        t = torch.empty(shape, dtype=dtype, device=device)
-    if returned:
-        t.record_stream(torch.cuda.current_stream(device))
-    return t
 
 
 def _workspace(workspace, need, device, stream):

@@ -14,13 +14,12 @@ are other paths -- and anything else raises.
 """
 from __future__ import annotations
 
-import functools
 from typing import Optional
 
 import torch
 from torch import nn
 
-from ..kernels.kv_append import _dense_block_table, flash_attn_with_kvcache, rope_kv_append
+from ..kernels.kv_append import _dense_block_table, _on_stream, flash_attn_with_kvcache, rope_kv_append
 from ..kernels.prefill import gqa_fwd_batch_prefill
 
 
@@ -38,20 +37,6 @@ def _set_cos_sin_cache(inv_freq: torch.Tensor, max_length: int):
     t = torch.arange(max_length, device=inv_freq.device, dtype=inv_freq.dtype)
     freqs = torch.outer(t, inv_freq)
     return torch.cat((freqs.cos(), freqs.sin()), dim=-1).to(torch.float32).contiguous()
-
-
-def _on_stream(method):
-    """``method`` with ``stream=``: all of its work on that stream, projections included; the caller orders the stream behind
-    what the arguments need and what uses the result behind it."""
-    @functools.wraps(method)
-    def call(self, *args, stream=None, **kw):
-        if stream is None:
-            return method(self, *args, **kw)
-        with torch.cuda.stream(stream):
-            out = method(self, *args, **kw)
-        out.record_stream(torch.cuda.current_stream(out.device))
-        return out
-    return call
 
 
 class TP_Attn:

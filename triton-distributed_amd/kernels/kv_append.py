@@ -180,15 +180,16 @@ def apply_rotary_pos_emb(x: torch.Tensor, cos_sin: torch.Tensor, position_ids: t
                           position_ids=position_ids, q=x)
 
 
-_ARANGE = {}
+_ARANGE = {}   # tables of dense caches by device, stream (each is filled on the stream that reads it) and rows
 
 
 def _dense_block_table(device, n):
-    key = (device.index, n)
+    key = (device.index, stream_handle(None, device.index), n)
     t = _ARANGE.get(key)
     if t is None:
         t = torch.arange(n, dtype=torch.int32, device=device).view(n, 1)
-        _ARANGE[key] = t
+        if not torch.cuda.is_current_stream_capturing():   # (while a graph is captured nothing fills it: the graph's own)
+            _ARANGE[key] = t
     return t
 
 

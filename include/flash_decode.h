@@ -523,9 +523,10 @@ FD_API int fd_kv_append(void* stream, const void* k_new, const void* v_new, void
  *  keys, packed [total_k, Hkv, D]         (block_table NULL) sequence b's keys are cu_seqlens_k[b] .. [b + 1] - 1
  *  keys, paged  [num_pages, P, Hkv, D]    (block_table given) kv_lens[b] tokens, new ones included
  *  x[i, j] = sm_scale * q_i . k_j, soft-capped if params.soft_cap > 0; row i of n_q sees the keys j < n_k and, causal,
- *  j <= i + n_k - n_q: the last row sees the last key, whatever the lengths.  A row that sees nothing gets out = 0,
- *  lse = -inf.  Rows that belong to no sequence (behind the last one, before the first, behind q_lens[b]) are left as
- *  they are.  What lies behind a sequence's last key is not read.
+ *  j <= i + n_k - n_q: the last row sees the last key, whatever the lengths.  Of a sequence that is longer than its table
+ *  (kv_lens[b] > max_pages_per_seq * P) the rows stand where they would, behind the keys that there are.  A row that sees
+ *  nothing gets out = 0, lse = -inf.  Rows that belong to no sequence (behind the last one, before the first, behind
+ *  q_lens[b]) are left as they are.  What lies behind a sequence's last key is not read.
  *  No device value can lead a kernel out of bounds: offsets, lengths and page ids are clamped.
  */
 typedef struct fd_prefill_args {

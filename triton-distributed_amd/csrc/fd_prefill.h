@@ -2,7 +2,7 @@
 // tokens, and the prefix part of a shared-prefix decode step.
 //
 // out[i,h] = sum_j softmax_j(scale q[i,h].k[j,h/G]) v[j,h/G] over the keys j that row i sees: j < n_k, and in the causal
-// form j <= i + n_k - n_q (the last query sees the last key).  One pass over the keys with the running maximum m and sum
+// form j <= i + n_k - n_q (the last query sees the last key; a length beyond the table's room counts in full here).  One pass over the keys with the running maximum m and sum
 // l of the softmax; the accumulator is rescaled only when the maximum has grown by more than 2^8 (as in
 // fd_softmax_step).
 //
@@ -118,6 +118,7 @@ struct PrefillTile {
 // of its keys.
 struct PrefillItem {
   int kvh, q_start, n_q, j, k_start, n_k, slot, split, splits, min_tiles, causal;
+  int ahead;                 // causal: token i of the rows stands behind i + ahead keys
   const int32_t* table;      // nullptr: packed keys from k_start on
 
   // keys that row r of the sequence sees: [0, limit_of(r))
@@ -125,7 +126,7 @@ struct PrefillItem {
     return (int)(((uint64_t)(uint32_t)r * a.g_magic) >> a.g_shift);
   }
   __device__ __forceinline__ int limit_of(const PrefillArgs& a, int r) const {
-    return causal ? min(n_k, token_of(a, r) + 1 + n_k - n_q) : n_k;
+    return causal ? min(n_k, token_of(a, r) + 1 + ahead) : n_k;
   }
   // The token row of the pool that holds key `tok` (any value: keys past the last one repeat it); `entry`: its page, so that
   // the table can be read ahead of its use.
@@ -209,7 +210,7 @@ __device__ __forceinline__ bool fd_find_item(const PrefillArgs& a, int bm, Prefi
     it.q_start = b0 + w;
     it.n_k = __builtin_amdgcn_readlane(keys, w);
     it.n_q = 1;
-    it.causal = 0;
+    it.causal = it.ahead = 0;
     it.table = a.own_bt + (int64_t)it.q_start * a.own_sbt;
     return true;
   }
@@ -222,14 +223,15 @@ __device__ __forceinline__ bool fd_find_item(const PrefillArgs& a, int bm, Prefi
   // sequence from its end, where a causal row sees the most -- short work fills in behind long.
   for (int b0 = 0, base = 0; b0 < a.batch; b0 += 64) {
     const int mine = b0 + lane;
-    int qs = 0, nq = 0, ks = 0, nk = -1, tiles = 0;
+    int qs = 0, nq = 0, ks = 0, nk = -1, length = 0, tiles = 0;
     if (mine < a.batch) {
       fd_prefill_span(a, mine, qs, nq);
       if (a.bt) {
-        nk = min(max(a.kv_lens[mine], 0), a.max_pages * a.P);
+        length = max(a.kv_lens[mine], 0);         // what the table has no room for counts for the rows' places
+        nk = min(length, a.max_pages * a.P);
       } else {
         ks = min(max(a.cu_k[mine], 0), a.total_k);
-        nk = min(max(a.cu_k[mine + 1], ks), a.total_k) - ks;
+        nk = length = min(max(a.cu_k[mine + 1], ks), a.total_k) - ks;
       }
       tiles = (nq * a.G + bm - 1) / bm;
     }
@@ -242,6 +244,7 @@ __device__ __forceinline__ bool fd_find_item(const PrefillArgs& a, int bm, Prefi
       it.n_q = __builtin_amdgcn_readlane(nq, w);
       it.k_start = __builtin_amdgcn_readlane(ks, w);
       it.n_k = __builtin_amdgcn_readlane(nk, w);
+      it.ahead = __builtin_amdgcn_readlane(length, w) - it.n_q;
       it.j = __builtin_amdgcn_readlane(tiles, w) - 1 - __builtin_amdgcn_readlane(place, w);
       it.table = a.bt ? a.bt + (int64_t)(b0 + w) * a.sbt : nullptr;
       return true;

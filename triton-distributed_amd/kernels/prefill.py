@@ -123,7 +123,8 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
 
     * in the paged pools ``k``, ``v`` ``[pages, P, Hkv, D]`` (the query's type, or fp8-e4m3 with ``k_scale`` / ``v_scale``
       ``[Hkv]``): ``kv_lens[b]`` tokens of row ``b`` of ``block_table`` (int32 ``[B, max_pages]``), the new ones included
-      -- append first; or
+      -- append first; a length beyond the table's room means the keys that there are, with the causal limits of the full
+      length; or
     * with ``block_table=None`` and ``kv_lens=None`` packed in ``k``, ``v`` ``[total_k, Hkv, D]``: rows
       ``cu_seqlens_k[b] .. cu_seqlens_k[b + 1] - 1`` (default: ``cu_seqlens_q``).
 

@@ -113,7 +113,8 @@ class TP_Attn:
         offsets -- a whole prompt, or the next chunk of one.  Their K/V are appended in one launch (norms, rotary and fp8
         included), then causal attention covers cache and chunk.  ``q_lens`` (int32 ``[B]``): a batch padded to T, only the
         first ``q_lens[b]`` tokens of sequence b are real; what the padding wrote behind a sequence's length is
-        overwritten by its next tokens, and its rows of the result mean nothing.  The caller advances the offsets
+        overwritten by its next tokens, and its rows of the result mean nothing, nor do those of tokens that the sequence's
+        table has no room for (they are not stored).  The caller advances the offsets
         (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  ``stream=``: the whole block runs there; other keywords
         go to ``gqa_fwd_batch_prefill``."""
         bsz, q_len, _ = x.size()
@@ -126,15 +127,18 @@ class TP_Attn:
         k_norm = (self.k_norm_w, self.k_norm_eps) if hasattr(self, "k_norm_eps") else None
         k_cache, v_cache, kv_offset = kv_cache.update_kv_cache(k, v, layer_idx)
         table = kv_cache.block_table if kv_cache.block_table is not None else _dense_block_table(x.device, bsz)
-        kv_lens = torch.empty_like(kv_offset)
         prep_q = cos_sin_cache is not None or q_norm is not None
         q_rows = torch.empty(q.shape, dtype=q.dtype, device=q.device) if prep_q else q
-        rope_kv_append(k, v, k_cache, v_cache, table, kv_offset, kv_lens_out=kv_lens, k_scale=kv_cache.k_scale,
+        rope_kv_append(k, v, k_cache, v_cache, table, kv_offset, k_scale=kv_cache.k_scale,
                        v_scale=kv_cache.v_scale, cos_sin=cos_sin_cache, position_ids=position_ids,
                        q=q if prep_q else None, q_out=q_rows if prep_q else None, q_norm=q_norm, k_norm=k_norm)
         out = None
-        if q_lens is not None:
-            kv_lens = torch.minimum(kv_offset + q_lens, kv_lens)
+        # (not the append's grown lengths, which end at the table's room: tokens behind it were not stored, and the others keep
+        # their places)
+        if q_lens is None:
+            kv_lens = kv_offset + q_len
+        else:
+            kv_lens = kv_offset + q_lens.clamp(max=q_len)
             out = torch.zeros(bsz * q_len, q.shape[2], self.head_dim, dtype=q.dtype, device=q.device)
         starts = torch.arange(0, bsz * q_len + 1, q_len, dtype=torch.int32, device=x.device)
         out = gqa_fwd_batch_prefill(q_rows.reshape(bsz * q_len, -1, self.head_dim), k_cache, v_cache, starts, kv_lens, table,

@@ -216,9 +216,10 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     ``kv_lens_out`` receives ``cache_seqlens + T``.  ``num_splits`` 0 lets the library choose.
     ``shared_prefix`` = ``(prefix_lens, prefix_table, group_starts or None)``: sequences that share prefixes
     (``gqa_fwd_batch_decode_shared_prefix``); ``block_table`` and ``cache_seqlens`` then describe what each
-    sequence holds behind its group's prefix.
-    Not covered, and refused: more than one query token (``gqa_fwd_batch_prefill``), flash-attn's own rotary arguments, left padding,
-    sliding windows and ALiBi.
+    sequence holds behind its group's prefix, the library chooses the ranges of both (``num_splits`` 0), and of the decode's
+    keywords ``max_kv_len`` applies, with ``max_prefix_len`` beside it.
+    Not covered, and refused before anything is appended: more than one query token (``gqa_fwd_batch_prefill``),
+    flash-attn's own rotary arguments, left padding, sliding windows and ALiBi.
     """
     if q.dim() != 4 or q.shape[1] != 1:
         raise NotImplementedError("flash_attn_with_kvcache: this library covers the decode step (seqlen_q == 1)")
@@ -228,6 +229,12 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
         raise NotImplementedError("flash_attn_with_kvcache: cache_leftpad, alibi_slopes and window_size")
     if cache_seqlens is None:
         raise RuntimeError("flash_attn_with_kvcache: cache_seqlens is required")
+    if shared_prefix is not None:
+        if num_splits > 0:
+            raise NotImplementedError("flash_attn_with_kvcache: num_splits with shared_prefix (the library chooses)")
+        unknown = sorted(set(decode_kw) - {"max_kv_len", "max_prefix_len"})
+        if unknown:
+            raise TypeError(f"flash_attn_with_kvcache: {unknown[0]} does not go with shared_prefix")
     bsz, _, q_heads, head_dim = q.shape
     dev = q.device
     if isinstance(cache_seqlens, int):

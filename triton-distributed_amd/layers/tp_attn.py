@@ -39,6 +39,9 @@ def _set_cos_sin_cache(inv_freq: torch.Tensor, max_length: int):
     return torch.cat((freqs.cos(), freqs.sin()), dim=-1).to(torch.float32).contiguous()
 
 
+_PREFILL_KEYWORDS = {"soft_cap", "causal", "lse_out", "workspace", "max_kv_len", "kv_split"}
+
+
 class TP_Attn:
     """Attention block; QKV weights column-sharded over heads, output weights row-sharded (world_size 1 here)."""
 
@@ -115,8 +118,11 @@ class TP_Attn:
         first ``q_lens[b]`` tokens of sequence b are real; what the padding wrote behind a sequence's length is
         overwritten by its next tokens, and its rows of the result mean nothing, nor do those of tokens that the sequence's
         table has no room for (they are not stored).  The caller advances the offsets
-        (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  ``stream=``: the whole block runs there; other keywords
-        go to ``gqa_fwd_batch_prefill``."""
+        (``kv_cache.inc_offset(T)``, or ``inc_offset(q_lens)``).  ``stream=``: the whole block runs there; ``soft_cap``,
+        ``causal``, ``lse_out``, ``workspace``, ``max_kv_len`` and ``kv_split`` go to ``gqa_fwd_batch_prefill``."""
+        unknown = sorted(set(prefill_kw) - _PREFILL_KEYWORDS)
+        if unknown:      # (before anything is appended)
+            raise TypeError(f"TP_Attn.prefill: unexpected keyword {unknown[0]}")
         bsz, q_len, _ = x.size()
         if q_len == 0:
             return x.new_empty(bsz, 0, self.wo.shape[0])

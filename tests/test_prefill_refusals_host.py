@@ -28,3 +28,33 @@ def test_prefill_keywords_are_refused_before_the_append(fd):
     for name in ("output", "cu_seqlens_k", "k_scale", "no_such_keyword"):
         with pytest.raises(TypeError, match="unexpected keyword " + name):
             attn.prefill(torch.zeros(2, 3, 8), None, None, None, 0, **{name: 1})
+
+
+def test_arguments_with_derivatives(fd):
+    """Reverse mode while autograd records, forward mode always; queries, caches and fp8 scales alike."""
+    from torch.autograd import forward_ad
+    mk = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    i32 = lambda *s: mk(*s, dt=torch.int32)  # noqa: E731
+
+    def pre(q=mk(4, 8, 128), k=mk(6, 16, 2, 128), v=mk(6, 16, 2, 128), **kw):
+        return fd.gqa_fwd_batch_prefill(q, k, v, i32(3), i32(2), i32(2, 4), 0.1, **kw)
+
+    def shared(q=mk(4, 8, 128), k=mk(6, 16, 2, 128), v=mk(6, 16, 2, 128), **kw):
+        return fd.gqa_fwd_batch_decode_shared_prefix(q, k, v, None, None, i32(4), i32(4, 2), i32(1), i32(1, 2), 0.1, **kw)
+
+    for call in (pre, shared):
+        for name, shape, dt in (("q", (4, 8, 128), torch.bfloat16), ("k", (6, 16, 2, 128), torch.bfloat16),
+                                ("v", (6, 16, 2, 128), torch.bfloat16), ("k_scale", (2,), torch.float32),
+                                ("v_scale", (2,), torch.float32)):
+            other = {n: mk(2, dt=torch.float32) for n in ("k_scale", "v_scale")} if "scale" in name else {}
+            leaf = mk(*shape, dt=dt).requires_grad_()
+            with pytest.raises(RuntimeError, match="no backward"):
+                call(**{**other, name: leaf})
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):      # allowed: the next check answers
+                call(**{**other, name: leaf})
+            with forward_ad.dual_level(), torch.no_grad():
+                dual = forward_ad.make_dual(mk(*shape, dt=dt), mk(*shape, dt=dt))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(**{**other, name: dual})
+                with pytest.raises(RuntimeError, match="no CPU path"):
+                    call(**other)

@@ -8,7 +8,8 @@ share a prefix.
 
 Every function enqueues hand-written HIP kernels through the C ABI in ``include/flash_decode.h`` (``fd_prefill``,
 ``fd_decode_shared``); nothing synchronises with the host, lengths are never read on it, and there is no CPU path.  Forward
-only: a query, key or value that requires a gradient is refused while autograd records.
+only: a query, key, value or fp8 scale that requires a gradient is refused while autograd records, one with a forward-mode
+tangent always.
 
 ``stream=`` enqueues a call's kernels there instead of on the current stream.  The caller orders it behind what the arguments
 need and what uses the result behind it, and keeps the arguments alive; what the call allocates needs no ordering.
@@ -19,6 +20,7 @@ from ctypes import byref
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .._lib import (FD_COMBINE_SPLIT, FdParams, FdPrefillArgs, FdSharedArgs, check, fd_dtype_of, load_library,
                     stream_handle)
@@ -49,9 +51,18 @@ def _check_scales(name, k_scale, v_scale, kv_heads):
               f"{name}: fp8 scales are contiguous float32 tensors of {kv_heads} values")
 
 
-def _check_no_grad(name, q, k, v):
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
+def _check_no_grad(name, *tensors):
+    """No argument (queries, keys, values, fp8 scales) that a derivative goes through, in either mode."""
+    backward = torch.is_grad_enabled()
+    forward = getattr(forward_ad, "_current_level", 0) >= 0     # (outside every dual level nothing carries a tangent)
+    if backward or forward:
+        for t in tensors:
+            if t is None:
+                continue
+            if backward and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
+            if forward and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative: an argument carries a tangent")
 
 
 def _check_pool(name, q, k_cache, v_cache):
@@ -138,7 +149,7 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     library choose how many key ranges a row tile is cut into (more than one where there are few rows), else exactly that
     many, up to 64.
     """
-    _check_no_grad("gqa_fwd_batch_prefill", q, k, v)
+    _check_no_grad("gqa_fwd_batch_prefill", q, k, v, k_scale, v_scale)
     scale, soft_cap, causal = float(scale), float(soft_cap or 0.0), bool(causal)   # (values: a tensor could change under the key)
     key = (_sig(q), _sig(k), _sig(v), _sig(cu_seqlens_q), _sig(kv_lens), _sig(block_table), _sig(cu_seqlens_k), _sig(q_lens),
            _sig(output), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, causal, max_kv_len, kv_split)
@@ -255,7 +266,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     group's query heads.  ``q_lens`` is accepted and ignored, ``workspace`` used if it is large enough, as there; 16-bit
     queries with a cache of the same type or fp8-e4m3.  ``max_kv_len`` / ``max_prefix_len``: host-side hints.
     """
-    _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache)
+    _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache, k_scale, v_scale)
     scale, soft_cap = float(scale), float(soft_cap or 0.0)
     # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
     hints = (-(-max_kv_len // 1024) * 1024 if max_kv_len else 0, -(-max_prefix_len // 1024) * 1024 if max_prefix_len else 0)

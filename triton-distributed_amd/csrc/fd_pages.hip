@@ -73,12 +73,11 @@ __device__ __forceinline__ int for_free_pages(const int32_t* refs, int num_pages
 // ---------------------------------------------------------------- copy
 
 // Workgroups walk the (entry, layer, pool, piece) items of a list of page copies.  count: entries, or count_at: where they
-// are counted on the device.  tokens: nullptr (whole pages), or how many tokens of each entry's page.
+// are counted on the device.
 struct CopyJob {
   PagePool pool;
   const int32_t* src;
   const int32_t* dst;
-  const int32_t* tokens;
   const int32_t* count_at;
   int32_t count, pieces;
   int64_t piece_bytes;
@@ -95,8 +94,7 @@ __device__ __forceinline__ void copy_pages(const CopyJob& c, int wg, int wgs) {
     const int which = rest & 1, layer = rest >> 1;
     const int s = c.src[entry], d = c.dst[entry];
     if (s < 0 || s >= c.pool.num_pages || d < 0 || d >= c.pool.num_pages || s == d) continue;
-    int64_t bytes = c.pool.page_bytes[which];
-    if (c.tokens) bytes = bytes / c.pool.page_size * c.tokens[entry];
+    const int64_t bytes = c.pool.page_bytes[which];
     const int64_t first = piece * c.piece_bytes;
     const int64_t last = first + c.piece_bytes < bytes ? first + c.piece_bytes : bytes;
     char* base = c.pool.base[which] + layer * c.pool.layer_stride[which];

@@ -613,16 +613,18 @@ FD_API int fd_pages_copy(void* stream, const fd_page_pool* pool, const int32_t* 
                          int32_t count);
 
 /* Gives row b the pages that kv_lens[b] + new_tokens[b] tokens need (new_tokens NULL: `uniform` for every row).  ok[b]: 1, or
- * 0 where the table is too narrow or the pool has run out by then -- such a row keeps what it had.  Rows are served in
- * order, and a row that gets nothing still counts against the rows behind it.  batch <= 4096, and at most 2^20 new pages a
- * row (a row that wants more is refused). */
+ * 0 where the table is too narrow, the pool has run out by then, or the row wants tokens but lacks a page for those that
+ * kv_lens[b] counts already (a refusal that was not heeded, an idle row that was counted on) -- such a row keeps what it
+ * had.  Rows are served in order, and a row that gets nothing for want of free pages still counts against the rows behind it.
+ * batch <= 4096, and at most 2^20 new pages a row (a row that wants more is refused). */
 FD_API int fd_pages_reserve(void* stream, const fd_page_tables* tables, int32_t num_pages, int32_t page_size,
                             const int32_t* new_tokens, int32_t uniform, int32_t* ok);
 
 /* Makes row children[i] a fork of row parents[i]: same length, the parent's full pages shared (their counts go up), the
  * tokens of a part-filled last page copied to a fresh page of its own in every layer, so that both rows can be appended
- * to.  ok[i]: 1, or 0 where the fork is refused and nothing changes: a row out of range, a child that is its own parent, that
- * holds tokens or pages or was named before in the list, no free page left.  Parents count as they are before the call.
+ * to.  ok[i]: 1, or 0 where the fork is refused and nothing changes: a row out of range, a parent without a page for tokens
+ * that its length counts, a child that is its own parent, that holds tokens or pages or was named before in the list, no
+ * free page left.  Parents count as they are before the call.
  * workspace: fd_pages_workspace_bytes(num_pages, count) bytes. */
 FD_API int fd_pages_fork(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, const int32_t* parents,
                          const int32_t* children, int32_t count, int32_t* ok, void* workspace, int64_t workspace_bytes);

@@ -1,0 +1,45 @@
+"""Page operators on caches whose lengths and pages do not match, and at the limits of a call."""
+import pytest
+import torch
+
+from test_gpu_pages import DEV, Pair
+
+pytestmark = pytest.mark.gpu
+
+
+def advance(t, rows, n):
+    """Lengths go up without a word to the page operators."""
+    for r in rows:
+        t.lens[r] += n
+        t.m.lens[r] += n
+
+
+def test_a_length_without_pages_is_not_granted_more(fd):
+    """A refusal that was not heeded and an idle row that was counted on: what their lengths count has no pages, so an append
+    behind it would have a table with holes."""
+    t = Pair(fd, 1, 6, 16, 4, 8)
+    t.grow([48, 32, 0, 0])                                   # five of six pages
+    assert t.reserve([16, 17, 0, 0]) == [1, 0, 0 + 1, 1]     # row 1 wants two pages, none is left
+    advance(t, [0, 1, 2], 16)                                # row 1 and the idle row 2 go on all the same
+    t.free([3])
+    t.free([0])                                              # pages are free again
+    before = t.table.clone(), t.refs.clone()
+    ask = lambda new: fd.paged_kv_reserve(t.table, t.lens, t.refs, t.i32(new), 16).tolist()  # noqa: E731
+    assert ask([0, 1, 1, 0]) == [1, 0, 0, 1]
+    assert ask([0, 40, 17, 0]) == [1, 0, 0, 1]
+    assert ask([0, 0, 0, 0]) == [1, 1, 1, 1]                 # nothing wanted, nothing to refuse
+    assert torch.equal(t.table, before[0]) and torch.equal(t.refs, before[1])
+    got = fd.paged_kv_fork(t.k, t.v, t.table, t.lens, t.refs, t.i32([1, 2]), t.i32([0, 3]))
+    assert got.tolist() == [0, 0]                            # nor do they have all that a fork would share
+    assert torch.equal(t.table, before[0]) and torch.equal(t.refs, before[1]) and t.lens.tolist() == [0, 48, 16, 0]
+    t.free([1, 2])
+    t.reserve([16, 0, 33, 0])                                # freed, they are rows like any other
+
+
+def test_a_part_filled_page_that_is_missing(fd):
+    """The next token would go into the page that the row lacks."""
+    t = Pair(fd, 1, 8, 16, 2, 8)
+    t.grow([16, 0])
+    advance(t, [0, 1], 3)
+    ok = fd.paged_kv_reserve(t.table, t.lens, t.refs, 1, 16)
+    assert ok.tolist() == [0, 0] and t.table.tolist() == [[0] + [-1] * 7, [-1] * 8] and int(t.refs.sum()) == 1

@@ -134,6 +134,12 @@ constexpr int kMaxReservePages = 1 << 20;     // of a row and call: 1024 rows' w
 constexpr int kWantedEnough = (1 << 30) - 1;  // ... and sums of more than any pool holds stop here
 constexpr int kNothingMissing = 0x7fffffff;
 
+// Whether row b holds the page of its last token, and with it, from the front, those of all `len` (at most width * P): not
+// where tokens were counted that no page had been granted for.
+__device__ __forceinline__ bool holds_length(const PageTables& t, int b, int len, int P) {
+  return len == 0 || t.bt[b * t.sbt + (len - 1) / P] >= 0;
+}
+
 __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const PageTables t, int num_pages, int P,
                                                                        const int32_t* __restrict__ new_tokens, int uniform,
                                                                        int32_t* __restrict__ ok) {
@@ -146,8 +152,8 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_reserve_kernel(const Pa
     const int len = max(t.kv_lens[b], 0);
     const int64_t grown = (int64_t)len + max(new_tokens ? new_tokens[b] : uniform, 0);
     const int64_t last = (grown + P - 1) / P;
-    int missing = -1, first = 0;              // -1: refused, the table has no room
-    if (last <= t.width) {
+    int missing = -1, first = 0;              // -1: refused, the table has no room or lacks pages that the length counts on
+    if (last <= t.width && (grown == len || holds_length(t, b, len, P))) {
       first = (int)(((int64_t)len + P - 1) / P);
       int have = 0;
       for (int j = first + lane; j < (int)last; j += 64) have += t.bt[b * t.sbt + j] >= 0 ? 1 : 0;
@@ -213,7 +219,10 @@ __global__ void __launch_bounds__(kScanThreads) fd_pages_fork_plan_kernel(const 
       const int p = parents[i], c = children[i];
       bool good = p >= 0 && p < t.batch && c >= 0 && c < t.batch && p != c && t.kv_lens[c] == 0 && t.bt[c * t.sbt] < 0;
       for (int j = 0; good && j < i; ++j) good = children[j] != c;    // a row that was named before
-      if (good) len = (int)min((int64_t)max(t.kv_lens[p], 0), (int64_t)t.width * P);
+      if (good) {
+        len = (int)min((int64_t)max(t.kv_lens[p], 0), (int64_t)t.width * P);
+        if (!holds_length(t, p, len, P)) len = -1;
+      }
     }
     const int need = len > 0 && len % P ? 1 : 0;
     int total;

@@ -97,9 +97,10 @@ def paged_kv_copy(k_cache, v_cache, src_pages, dst_pages, *, stream=None):
 def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, torch.Tensor], page_size: int, *,
                      ok_out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
     """Gives every row the pages that its next ``new_tokens`` tokens need (an int for all rows, or int32 ``[B]``), so that
-    the append that follows has somewhere to write.  Returns int32 ``[B]``: 1, or 0 where the table is too narrow or the
-    pool has run out -- that row keeps what it had.  Rows are served in order; a row that gets nothing still counts against
-    the rows behind it.  At most 4096 rows, and 2^20 new pages a row."""
+    the append that follows has somewhere to write.  Returns int32 ``[B]``: 1, or 0 where the table is too narrow, the pool has
+    run out, or the row wants tokens but lacks a page for those that its length counts already (its length went up
+    without pages: free it first) -- that row keeps what it had.  Rows are served in order; a row that gets nothing for want of
+    free pages still counts against the rows behind it.  At most 4096 rows, and 2^20 new pages a row."""
     each = new_tokens if isinstance(new_tokens, torch.Tensor) else None
     batch = block_table.shape[0]
     _, t = _checked("paged_kv_reserve", (), (block_table, kv_lens, page_refs),
@@ -119,7 +120,8 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
     """Makes row ``children[i]`` a fork of row ``parents[i]`` (int32 ``[n]``): the parent's length, its full pages shared
     (counted, not copied), and of a part-filled last page a copy of its own, in every layer -- both rows can be appended to
     afterwards.  Returns int32 ``[n]``: 1, or 0 where a fork is refused and nothing changes (a row out of range or its own
-    parent, a child that holds tokens or pages or was named before, no free page left).  Parents count as they are before
+    parent, a parent without a page for tokens that its length counts, a child that holds tokens or pages or was named
+    before, no free page left).  Parents count as they are before
     the call."""
     n = parents.numel()
     pool, t = _checked("paged_kv_fork", (k_cache, v_cache), (block_table, kv_lens, page_refs),

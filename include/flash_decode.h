@@ -624,7 +624,7 @@ FD_API int fd_pages_reserve(void* stream, const fd_page_tables* tables, int32_t 
  * tokens of a part-filled last page copied to a fresh page of its own in every layer, so that both rows can be appended
  * to.  ok[i]: 1, or 0 where the fork is refused and nothing changes: a row out of range, a parent without a page for tokens
  * that its length counts, a child that is its own parent, that holds tokens or pages or was named before in the list, no
- * free page left.  Parents count as they are before the call.
+ * free page left.  Parents count as they are before the call.  count <= 16384.
  * workspace: fd_pages_workspace_bytes(num_pages, count) bytes. */
 FD_API int fd_pages_fork(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, const int32_t* parents,
                          const int32_t* children, int32_t count, int32_t* ok, void* workspace, int64_t workspace_bytes);

@@ -43,3 +43,18 @@ def test_a_part_filled_page_that_is_missing(fd):
     advance(t, [0, 1], 3)
     ok = fd.paged_kv_reserve(t.table, t.lens, t.refs, 1, 16)
     assert ok.tolist() == [0, 0] and t.table.tolist() == [[0] + [-1] * 7, [-1] * 8] and int(t.refs.sum()) == 1
+
+
+def test_the_most_forks_of_a_call(fd):
+    """Every child named twice, the second time in vain; many steps of the plan's scans."""
+    n = 8192
+    t = Pair(fd, 1, 3 * n, 16, n + 4, 2, heads=1, dim=16)
+    for at, lens, pages in ((0, 17, [0, 1]), (1, 16, [2]), (2, 5, [3])):      # (more rows than a reserve takes)
+        for lens_of, table, refs in ((t.lens, t.table, t.refs), (t.m.lens, t.m.table, t.m.refs)):
+            lens_of[at] = lens
+            for j, page in enumerate(pages):
+                table[at, j], refs[page] = page, 1
+    parents = [i % 4 for i in range(n)] + [0] * n
+    children = [4 + (i * 5) % n for i in range(n)] + [4 + i for i in range(n)]
+    assert len(parents) == 16384
+    assert t.fork(parents, children) == [1] * n + [0] * n

@@ -58,3 +58,15 @@ def test_arguments_with_derivatives(fd):
                     call(**{**other, name: dual})
                 with pytest.raises(RuntimeError, match="no CPU path"):
                     call(**other)
+
+
+def test_the_most_forks_of_a_call(fd):
+    import ctypes
+    L, lib = fd._lib, fd.load_library()
+    p, t = L.FdPagePool(), L.FdPageTables()
+    p.k_cache = p.v_cache = t.block_table = t.kv_lens = t.page_refs = 0x10000
+    p.k_page_bytes = p.v_page_bytes = p.k_page_stride = p.v_page_stride = 4096
+    p.layers, p.num_pages, p.page_size, t.stride_table_bs, t.max_pages_per_seq, t.batch = 1, 8, 16, 4, 4, 40000
+    n = 16385
+    assert lib.fd_pages_fork(None, ctypes.byref(p), ctypes.byref(t), 0x10000, 0x10000, n, 0x10000, 0x10000, 12 * n) == -5
+    assert b"16384" in lib.fd_last_error()

@@ -1480,6 +1480,8 @@ int fd_decode_shared(void* stream, const fd_shared_args* a) {
 
 namespace {
 
+constexpr int kMaxForks = 16384;   // a call's plan compares every child with those before it, in one workgroup: 13 ms
+
 int page_pool(const char* fn, const fd_page_pool* in, PagePool* out) {
   if (!in) return fail(FD_ERR_INVALID_ARG, "%s: pool is NULL", fn);
   if (!in->k_cache || !in->v_cache) return fail(FD_ERR_INVALID_ARG, "%s: NULL cache pointer", fn);
@@ -1559,6 +1561,7 @@ int fd_pages_fork(void* stream, const fd_page_pool* pool, const fd_page_tables* 
   if (int rc = page_tables(fn, tables, &t, true)) return rc;
   if (count < 0) return fail(FD_ERR_INVALID_ARG, "%s: count %d", fn, count);
   if (count == 0) return FD_OK;
+  if (count > kMaxForks) return fail(FD_ERR_TOO_LARGE, "%s: %d forks (at most %d a call)", fn, count, kMaxForks);
   if (!parents || !children || !ok) return fail(FD_ERR_INVALID_ARG, "%s: NULL list", fn);
   if (int rc = check_workspace(fn, workspace, workspace_bytes, fd_pages_workspace_bytes(pp.num_pages, count), 16)) return rc;
   return page_result(fn, fd_launch_pages_fork((hipStream_t)stream, pp, t, parents, children, count, ok, (int32_t*)workspace));

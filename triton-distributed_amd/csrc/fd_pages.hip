@@ -9,7 +9,9 @@
 // pool's reference counts is 4 bytes a page, in 16 KB steps that end as soon as enough free pages are found.  Measured
 // on caches of four layers, pages of 16 tokens x 8 heads of 128 in bf16: a copy of 777 of them 81 us = 5.0 TB/s, a compaction
 // that moves 442 MB 95 us = 4.6 TB/s (a plain 1 GiB copy: 5.1 TB/s); freeing and forking 64 rows is bound by the host's
-// part of two calls (21 us).
+// part of two calls (21 us).  The one-workgroup plans grow with what they look at: a reserve that finds nothing free 8 us in
+// a pool of 4096 pages, 31 us in 65536, 0.41 ms in 2^20; a fork's plan, which compares every child with those before it,
+// 84 us for 1024 forks, 0.9 ms for 4096, 13 ms for 16384 (the most that a call takes).
 #include "fd_common.h"
 
 namespace {

@@ -122,7 +122,7 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
     afterwards.  Returns int32 ``[n]``: 1, or 0 where a fork is refused and nothing changes (a row out of range or its own
     parent, a parent without a page for tokens that its length counts, a child that holds tokens or pages or was named
     before, no free page left).  Parents count as they are before
-    the call."""
+    the call.  At most 16384 forks."""
     n = parents.numel()
     pool, t = _checked("paged_kv_fork", (k_cache, v_cache), (block_table, kv_lens, page_refs),
                        (("parents", parents, (n,)), ("children", children, (n,)), ("ok_out", ok_out, (n,))))

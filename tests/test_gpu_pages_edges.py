@@ -58,3 +58,30 @@ def test_the_most_forks_of_a_call(fd):
     children = [4 + (i * 5) % n for i in range(n)] + [4 + i for i in range(n)]
     assert len(parents) == 16384
     assert t.fork(parents, children) == [1] * n + [0] * n
+
+
+def test_wild_tables_and_lists_stay_in_bounds(fd):
+    """Page ids, lengths, counts and rows far outside their ranges: nothing around the tables and pools changes."""
+    wild = [2 ** 31 - 1, -2 ** 31, -5, 100, 3, 0, 7, 99999]
+    around = dict(dtype=torch.int32, device=DEV)
+    whole = {name: torch.full((n + 512,), 123456, **around) for name, n in (("table", 32), ("lens", 4), ("refs", 8), ("ok", 4))}
+    table, lens, refs, ok = (whole[n][256:256 + s] for n, s in (("table", 32), ("lens", 4), ("refs", 8), ("ok", 4)))
+    table = table.view(4, 8)
+    pool = torch.zeros(10, 2, 8, 16, 1, 64, device=DEV)       # (slice 4: K, slice 5: V, zeros around them)
+    pool[4:6] = 1.0
+    lists = torch.tensor([wild[:4], wild[4:]], **around)
+    for round_ in range(4):
+        table.copy_(torch.tensor([wild, wild[::-1], [-1] * 8, [-1] * 8], **around))
+        lens.copy_(torch.tensor([[2 ** 31 - 1, -2 ** 31, 0, 40], [128, 129, -9, 5], [17, 33, 0, 0], [0, 0, 0, 0]][round_], **around))
+        refs.copy_(torch.tensor([0, -4, 2 ** 31 - 1, 1, 0, 0, -2 ** 31, 3], **around))
+        k, v = pool[4], pool[5]
+        for rows in lists:
+            fd.paged_kv_reserve(table, lens, refs, rows.abs().clamp(min=0), 16, ok_out=ok)
+            fd.paged_kv_fork(k, v, table, lens, refs, rows, rows.flip(0).contiguous(), ok_out=ok)
+            fd.paged_kv_copy(k, v, rows, rows.flip(0).contiguous())
+            fd.paged_kv_compact(k, v, table, refs)
+            fd.paged_kv_free(table, lens, refs, rows)
+            torch.cuda.synchronize()
+    for name, t in whole.items():
+        assert (t[:256] == 123456).all() and (t[-256:] == 123456).all(), name
+    assert not pool[:4].any() and not pool[6:].any() and (pool[4:6] == 1.0).all()

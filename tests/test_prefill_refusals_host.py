@@ -70,3 +70,23 @@ def test_the_most_forks_of_a_call(fd):
     n = 16385
     assert lib.fd_pages_fork(None, ctypes.byref(p), ctypes.byref(t), 0x10000, 0x10000, n, 0x10000, 0x10000, 12 * n) == -5
     assert b"16384" in lib.fd_last_error()
+
+
+def test_hints_and_splits_count_by_value(fd, monkeypatch):
+    """Given as tensors they may change in place between calls."""
+    import importlib
+    pre = importlib.import_module(fd.__name__ + ".kernels.prefill")
+    seen = []
+    monkeypatch.setattr(pre, "_prefill_image", lambda *a: (None, seen.append(a[-2:])))
+    monkeypatch.setattr(pre, "_shared_image", lambda *a: (None, seen.append(a[-1])))
+    mk = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    i32 = lambda *s: mk(*s, dt=torch.int32)  # noqa: E731
+    q, kv, a, b = mk(3, 8, 128), mk(6, 16, 2, 128), torch.tensor(5), torch.tensor(2)
+    for x, y in ((5, 2), (2000, 2), (2000, 3)):
+        a.fill_(x), b.fill_(y)
+        for _ in range(2):
+            fd.gqa_fwd_batch_prefill(q, kv, kv, i32(3), i32(2), i32(2, 4), 0.1, max_kv_len=a, kv_split=b)
+            fd.gqa_fwd_batch_decode_shared_prefix(q, kv, kv, None, None, i32(3), i32(3, 2), i32(1), i32(1, 2), 0.1,
+                                                  max_kv_len=a, max_prefix_len=b)
+    assert seen == [(5, 2), (1024, 1024), (2000, 2), (2048, 1024), (2000, 3)]
+    assert all(type(n) is int for pair in seen for n in pair)

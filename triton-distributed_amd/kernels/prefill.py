@@ -150,7 +150,9 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     many, up to 64.
     """
     _check_no_grad("gqa_fwd_batch_prefill", q, k, v, k_scale, v_scale)
-    scale, soft_cap, causal = float(scale), float(soft_cap or 0.0), bool(causal)   # (values: a tensor could change under the key)
+    # (values: a tensor could change under the key)
+    scale, soft_cap, causal = float(scale), float(soft_cap or 0.0), bool(causal)
+    max_kv_len, kv_split = int(max_kv_len or 0), int(kv_split)
     key = (_sig(q), _sig(k), _sig(v), _sig(cu_seqlens_q), _sig(kv_lens), _sig(block_table), _sig(cu_seqlens_k), _sig(q_lens),
            _sig(output), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, causal, max_kv_len, kv_split)
     cached = _PREFILL_CACHE.get(key)
@@ -189,7 +191,7 @@ def prefill_workspace_bytes(q, k, v, cu_seqlens_q, kv_lens, block_table, *, cu_s
                             max_kv_len=None, kv_split=0) -> int:
     """Bytes of workspace that ``gqa_fwd_batch_prefill`` uses for tensors of these shapes (0: none)."""
     return _prefill_image("prefill_workspace_bytes", q, k, v, cu_seqlens_q, kv_lens, block_table, 1.0, 0.0, True,
-                          cu_seqlens_k, None, None, None, k_scale, v_scale, max_kv_len, kv_split)[1]
+                          cu_seqlens_k, None, None, None, k_scale, v_scale, int(max_kv_len or 0), int(kv_split))[1]
 
 
 def _prefill_image(name, q, k, v, cu_q, kv_lens, block_table, scale, soft_cap, causal, cu_k, q_lens, output, lse_out,
@@ -240,7 +242,7 @@ def _prefill_image(name, q, k, v, cu_q, kv_lens, block_table, scale, soft_cap, c
     p.q_heads, p.kv_heads, p.head_dim, p.page_size, p.num_pages = q_heads, kv_heads, head_dim, page_size, num_pages
     p.max_pages_per_seq, p.q_dtype, p.kv_dtype = max_pages, fd_dtype_of(q), fd_dtype_of(k, fp8_bytes=k_scale is not None)
     p.out_dtype, p.soft_cap = p.q_dtype, float(soft_cap or 0.0)
-    p.max_kv_len, p.num_splits = int(max_kv_len or 0), int(kv_split)
+    p.max_kv_len, p.num_splits = max_kv_len, kv_split
     probe = FdPrefillArgs.from_buffer_copy(a)
     probe.block_table = 256 if paged else None    # whether there is a table is all that the size asks of it
     need = load_library().fd_prefill_workspace_bytes(byref(probe))
@@ -269,7 +271,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache, k_scale, v_scale)
     scale, soft_cap = float(scale), float(soft_cap or 0.0)
     # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
-    hints = (-(-max_kv_len // 1024) * 1024 if max_kv_len else 0, -(-max_prefix_len // 1024) * 1024 if max_prefix_len else 0)
+    hints = tuple(-(-int(n or 0) // 1024) * 1024 for n in (max_kv_len, max_prefix_len))
     key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(kv_lens), _sig(block_table), _sig(prefix_lens), _sig(prefix_table),
            _sig(group_starts), _sig(output_combine), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, hints)
     cached = _SHARED_CACHE.get(key)

@@ -600,7 +600,7 @@ typedef struct fd_page_pool {
 } fd_page_pool;
 
 typedef struct fd_page_tables {
-  int32_t* block_table;       /* [batch, max_pages_per_seq]                                                           */
+  int32_t* block_table;       /* [batch, max_pages_per_seq], rows apart from each other                               */
   int32_t* kv_lens;           /* [batch]                                                                              */
   int32_t* page_refs;         /* [num_pages]                                                                          */
   int64_t stride_table_bs;

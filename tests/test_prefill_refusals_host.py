@@ -90,3 +90,18 @@ def test_hints_and_splits_count_by_value(fd, monkeypatch):
                                                   max_kv_len=a, max_prefix_len=b)
     assert seen == [(5, 2), (1024, 1024), (2000, 2), (2048, 1024), (2000, 3)]
     assert all(type(n) is int for pair in seen for n in pair)
+
+
+def test_table_rows_that_overlap_are_refused(fd):
+    """A page operator writes the table: an expanded row, or windows of one, would be several rows at once."""
+    import ctypes
+    L, lib = fd._lib, fd.load_library()
+    t = L.FdPageTables()
+    t.block_table = t.kv_lens = t.page_refs = 0x10000
+    t.max_pages_per_seq, t.batch = 4, 3
+    for stride in (0, 3):
+        t.stride_table_bs = stride
+        assert lib.fd_pages_reserve(None, ctypes.byref(t), 8, 16, None, 1, 0x10000) == -1 and b"apart" in lib.fd_last_error()
+        assert lib.fd_pages_free(None, ctypes.byref(t), 8, 0x10000, 1) == -1 and b"apart" in lib.fd_last_error()
+    t.batch = 1                                                  # one row: its stride means nothing
+    assert lib.fd_pages_free(None, ctypes.byref(t), 8, None, 0) == 0

@@ -1511,6 +1511,9 @@ int page_tables(const char* fn, const fd_page_tables* in, PageTables* out, bool 
     return fail(FD_ERR_INVALID_ARG, "%s: NULL table pointer", fn);
   if (in->batch <= 0 || in->max_pages_per_seq <= 0 || in->stride_table_bs < 0)
     return fail(FD_ERR_INVALID_ARG, "%s: batch %d, max_pages_per_seq %d", fn, in->batch, in->max_pages_per_seq);
+  if (in->batch > 1 && in->stride_table_bs < in->max_pages_per_seq)   // (they are written: two rows would share entries)
+    return fail(FD_ERR_INVALID_ARG, "%s: table rows of %d entries, %lld apart", fn, in->max_pages_per_seq,
+                (long long)in->stride_table_bs);
   out->bt = in->block_table; out->kv_lens = in->kv_lens; out->refs = in->page_refs; out->sbt = in->stride_table_bs;
   out->batch = in->batch; out->width = in->max_pages_per_seq;
   return FD_OK;

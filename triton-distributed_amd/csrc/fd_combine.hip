@@ -23,13 +23,19 @@ constexpr int kCombineThreads = 256;
 constexpr int kMaxPartials = 1024;  // LSEs staged in LDS per pass
 constexpr int kPrefetch = 8;        // partial rows a thread requests before the weights are known
 
-// max of v[0..n) (LDS), the same value in every lane: a strided scan per lane, then a butterfly over the wave
+// The reference point of partials with the LSEs v[0..n) (LDS): their maximum, the same value in every lane -- a strided scan per
+// lane, then a butterfly over the wave.  -inf where nothing is valid.  The maximum drops NaN; where there is nothing else,
+// any finite value makes the weights of the NaN partials, and with them the row, NaN.
 __device__ __forceinline__ float wave_max_of(const float* v, int n) {
   float m = -INFINITY;
-  for (int i = threadIdx.x & 63; i < n; i += 64) m = fmaxf(m, v[i]);
+  bool nan = false;
+  for (int i = threadIdx.x & 63; i < n; i += 64) {
+    m = fmaxf(m, v[i]);
+    nan = nan || v[i] != v[i];
+  }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
-  return m;
+  return __any(nan) ? fmaxf(m, 0.f) : m;
 }
 
 template <int D>
@@ -194,10 +200,10 @@ __global__ void __launch_bounds__(kCombineThreads) fd_combine_kernel(const Combi
       float o = 0.f;
       for (int i = 0; i < NG; ++i) o += s_acc[i * ncol + tid];
       const float Lsum = lw;
-      const float inv = Lsum > 0.f ? 1.0f / Lsum : 0.f;
+      const float inv = Lsum != 0.f ? 1.0f / Lsum : 0.f;
       store_from_f32(dst, dst_base + col0 + tid, dst_dtype, o * inv);
       if (tid == 0 && col0 == 0) {
-        const float lse = Lsum > 0.f ? M_t + __logf(Lsum) : -INFINITY;
+        const float lse = Lsum != 0.f ? M_t + __logf(Lsum) : -INFINITY;
         if (lse_col) store_from_f32(dst, dst_base + D, dst_dtype, lse);
         if (lse_sep) *lse_sep = lse;
       }
@@ -280,6 +286,7 @@ __global__ void __launch_bounds__(kCombineThreads) fd_combine_own_kernel(const C
   float M = mine;
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+  if (__any(mine != mine)) M = fmaxf(M, 0.f);        // (as in wave_max_of)
   float L = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -305,11 +312,11 @@ __global__ void __launch_bounds__(kCombineThreads) fd_combine_own_kernel(const C
       v += s_acc[i][tid];
       Lsum += s_l[i];
     }
-    const float inv = Lsum > 0.f ? 1.0f / Lsum : 0.f;
+    const float inv = Lsum != 0.f ? 1.0f / Lsum : 0.f;
     const int64_t out_base = (int64_t)b * a.s_ob + (int64_t)h * a.s_oh;
     store_from_f32(a.out, out_base + col0 + tid, a.out_dtype, v * inv);
     if (tid == 0 && col0 == 0) {
-      const float res = Lsum > 0.f ? M + __logf(Lsum) : -INFINITY;
+      const float res = Lsum != 0.f ? M + __logf(Lsum) : -INFINITY;
       if (a.mode == FD_COMBINE_SPLIT_LSE) store_from_f32(a.out, out_base + D, a.out_dtype, res);
       if (a.lse_out) a.lse_out[(int64_t)b * a.Hq + h] = res;
     }

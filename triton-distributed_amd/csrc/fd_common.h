@@ -552,7 +552,8 @@ __device__ __forceinline__ void cta_merge_store_rounds(const SplitArgs& a, float
   const int pstep = a.hpw * stride;   // floats between the partials of two sub-ranges of one member
   const bool through = a.store_through != 0;
 
-  // ---- step 1: weights, 1 / L and the LSE of every row
+  // ---- step 1: weights, 1 / L and the LSE of every row.  L is 0 where there is no key and NaN where a score or a value is
+  // (the maximum drops NaN, so M alone does not tell).
   for (int row = tid; row < a.hpw * heads; row += nthreads) {
     int hm = 0;   // member of the row, without a division by a run-time value or a divergent loop (hpw <= 8)
 #pragma unroll
@@ -594,12 +595,12 @@ __device__ __forceinline__ void cta_merge_store_rounds(const SplitArgs& a, float
       case 8: weigh(std::integral_constant<int, 8>{}, 8); break;
       default: weigh(std::integral_constant<int, 0>{}, w.nsub);
     }
-    ml[HB] = L > 0.f ? 1.0f / L : 0.f;
+    ml[HB] = L != 0.f ? 1.0f / L : 0.f;
     const int kvh = a.member_hb ? w.kvh0 : w.kvh0 + (a.v_members == 2 ? hm >> 1 : hm);
     const int co = a.v_members == 2 ? (hm & 1) * 128 : 0;   // this member's half of the V columns
     const int hb = a.member_hb ? w.hb0 + hm : w.hb;
     if (h < a.G - hb * HB && co == 0 && (a.tickets || !a.no_lse)) {
-      const float lse = L > 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
+      const float lse = L != 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
       const int head = kvh * a.G + hb * HB + h;
       const int64_t lse_at = ((int64_t)w.b * a.Hq + head) * a.S + w.s;
       const int64_t col_d = (int64_t)w.b * a.so_b + (int64_t)head * a.so_h + (int64_t)w.s * a.so_s + a.dv;
@@ -717,13 +718,15 @@ __device__ __forceinline__ void cta_merge_store_one_round(const SplitArgs& a, co
           L += pp[HB * D + HB + h] * wgt;
           o += pp[h * D + d] * wgt;
         }
+      } else {                          // no key, or NaN scores only
+        for (int p = 0; p < w.nsub; ++p) L += part[(hm + a.hpw * p) * stride + HB * D + HB + h];
       }
-      const float inv = L > 0.f ? 1.0f / L : 0.f;
+      const float inv = L != 0.f ? 1.0f / L : 0.f;
       const int head = kvh * a.G + hb * HB + h;
       const int64_t row = (int64_t)w.b * a.so_b + (int64_t)head * a.so_h + (int64_t)w.s * a.so_s;
       store_partial1(a.out, row + d + co, a.mid_dtype, o * inv, a.store_through != 0);
       if (d == 0 && co == 0 && !a.no_lse) {
-        const float lse = L > 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
+        const float lse = L != 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
         if (a.lse) {
           a.lse[((int64_t)w.b * a.Hq + head) * a.S + w.s] = lse;
         } else {
@@ -772,6 +775,9 @@ __device__ __forceinline__ void cta_merge_store_one_round(const SplitArgs& a, co
           L += ll[p] * wgt;
           o += xx[p] * wgt;
         }
+      } else {                                   // no key, or NaN scores only
+#pragma unroll
+        for (int p = 0; p < NS; ++p) L += ll[p];
       }
     };
     switch (w.nsub) {
@@ -788,14 +794,16 @@ __device__ __forceinline__ void cta_merge_store_one_round(const SplitArgs& a, co
             L += pp[HB * D + HB + h] * wgt;
             o += *(const f32x4*)(pp + h * D + d) * wgt;
           }
+        } else {
+          for (int p = 0; p < w.nsub; ++p) L += part[(hm + a.hpw * p) * stride + HB * D + HB + h];
         }
     }
-    float inv = L > 0.f ? 1.0f / L : 0.f;
+    float inv = L != 0.f ? 1.0f / L : 0.f;
     o *= inv;
     const int head = kvh * a.G + hb * HB + h;
     const int64_t row = (int64_t)w.b * a.so_b + (int64_t)head * a.so_h + (int64_t)w.s * a.so_s;
     const int64_t off = row + d + co;
-    const float lse = L > 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
+    const float lse = L != 0.f ? (M + fd_log2(L)) * FD_LN2 : -INFINITY;
     if (a.tickets) {
       // fused combine (fp32 partials only): another XCD's workgroup may read these
 #pragma unroll
@@ -1061,7 +1069,12 @@ __device__ __forceinline__ void fused_combine(const SplitArgs& a, const WorkItem
     const int head = head0 + h;
     const float* ls = s_lse + h * NP;
     float M = -INFINITY;
-    for (int s = 0; s < NP; ++s) M = fmaxf(M, ls[s]);
+    bool nan = false;
+    for (int s = 0; s < NP; ++s) {
+      M = fmaxf(M, ls[s]);
+      nan = nan || ls[s] != ls[s];
+    }
+    if (nan) M = fmaxf(M, 0.f);                // (not "nothing valid": any finite reference makes the row NaN)
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float L = 0.f;
     if (M > -INFINITY) {
@@ -1094,12 +1107,12 @@ __device__ __forceinline__ void fused_combine(const SplitArgs& a, const WorkItem
         L += wgt;
       }
     }
-    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    const float inv = L != 0.f ? 1.0f / L : 0.f;
     const int64_t ob = (int64_t)w.b * a.sfo_b + (int64_t)head * a.sfo_h;
 #pragma unroll
     for (int k = 0; k < 4; ++k) store_from_f32(a.fout, ob + d + k, a.out_dtype, acc[k] * inv);
     if (d == 0) {
-      const float lse = L > 0.f ? M + __logf(L) : -INFINITY;
+      const float lse = L != 0.f ? M + __logf(L) : -INFINITY;
       if (a.lse_column) store_from_f32(a.fout, ob + D, a.out_dtype, lse);
       if (a.flse) a.flse[(int64_t)w.b * a.Hq + head] = lse;
     }

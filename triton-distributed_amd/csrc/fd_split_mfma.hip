@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(NB == 2 ? 256 : 512) FD_MFMA_OCC fd_split_mfma
       lsum += __shfl_xor(lsum, 32);
       const int h = 16 * nb + c;
       if (h < nheads) {
-        const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+        const float inv = lsum != 0.f ? 1.0f / lsum : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float v[8];
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(NB == 2 ? 256 : 512) FD_MFMA_OCC fd_split_mfma
           for (int j = 0; j < 8; ++j) v[j] = acc[nb][j][i] * inv;
           park_store8(slot + kHB * 4, h * kD + 32 * g + 8 * i, a.mid_dtype, v);
         }
-        if (g == 0) ((float*)slot)[h] = lsum > 0.f ? (m[nb] + fd_log2(lsum)) * FD_LN2 : -INFINITY;
+        if (g == 0) ((float*)slot)[h] = lsum != 0.f ? (m[nb] + fd_log2(lsum)) * FD_LN2 : -INFINITY;
       }
     }
   };

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(NB == 2 ? 256 : 512) fd_split_mfma_fp8_kernel(
       lsum += __shfl_xor(lsum, 32);
       const int h = 16 * nb + c;
       if (h < nheads) {
-        const float inv = lsum > 0.f ? v_scale / lsum : 0.f;
+        const float inv = lsum != 0.f ? v_scale / lsum : 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = 4 * g + i;
@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(NB == 2 ? 256 : 512) fd_split_mfma_fp8_kernel(
           for (int j = 0; j < 8; ++j) v[j] = acc[nb][j][i] * inv;
           park_store8(slot + kHB * 4, h * kD + 16 * (r & 7) + 8 * (r >> 3), a.mid_dtype, v);
         }
-        if (g == 0) ((float*)slot)[h] = lsum > 0.f ? (m[nb] + fd_log2(lsum)) * FD_LN2 : -INFINITY;
+        if (g == 0) ((float*)slot)[h] = lsum != 0.f ? (m[nb] + fd_log2(lsum)) * FD_LN2 : -INFINITY;
       }
     }
   };

@@ -108,7 +108,7 @@ typedef struct fd_params {
   int32_t kv_dtype;         /* fd_dtype of k_cache / v_cache                       */
   int32_t mid_dtype;        /* fd_dtype of the split partials (out_split / mid_o)  */
   int32_t out_dtype;        /* fd_dtype of the combined output                     */
-  float soft_cap;           /* <= 0: off                                           */
+  float soft_cap;           /* <= 0: off; a capped score is good to soft_cap * 2^-22 */
   const float* k_scale;     /* [Hkv] fp32 dequant scales, FD_FP8_E4M3 only         */
   const float* v_scale;     /* [Hkv]                                               */
   int32_t path;             /* fd_path                                             */
@@ -208,7 +208,8 @@ FD_API int fd_split_kv(void* stream, const void* q, const void* k_cache, const v
  *            partials the reference's allgather delivers from other ranks
  *            (sp_flash_decode_layer.py:136-145).
  *
- * A row with no valid partial yields out = 0, lse = -inf (the reference yields NaN).
+ * A row with no valid partial yields out = 0, lse = -inf (the reference yields NaN); one with a NaN LSE among its valid
+ * partials is NaN.
  */
 FD_API int fd_combine(void* stream, const void* mid_o, const float* mid_lse, void* out, float* lse_out,
                const int32_t* seqlens, int32_t batch, int32_t q_heads, int32_t num_partials,
@@ -526,7 +527,8 @@ FD_API int fd_kv_append(void* stream, const void* k_new, const void* v_new, void
  *  j <= i + n_k - n_q: the last row sees the last key, whatever the lengths.  Of a sequence that is longer than its table
  *  (kv_lens[b] > max_pages_per_seq * P) the rows stand where they would, behind the keys that there are.  A row that sees
  *  nothing gets out = 0, lse = -inf.  Rows that belong to no sequence (behind the last one, before the first, behind
- *  q_lens[b]) are left as they are.  What lies behind a sequence's last key is not read.
+ *  q_lens[b]) are left as they are.  What lies behind a sequence's last key is not read.  A row that meets a NaN -- its own,
+ *  a key's that it sees, a scale's -- is NaN in out and lse, however many ranges its keys are cut into.
  *  No device value can lead a kernel out of bounds: offsets, lengths and page ids are clamped.
  */
 typedef struct fd_prefill_args {
@@ -636,7 +638,7 @@ FD_API int fd_pages_free(void* stream, const fd_page_tables* tables, int32_t num
 
 /* Moves the live pages to the front of the pool: with n live pages, the k-th live page at or behind n goes to the k-th free
  * page before n, in every layer, counts and tables with it.  *live_out (device): n.  `tables` must hold every row that holds
- * pages. */
+ * pages; page ids kept anywhere else (a prefix_table of its own) are not rewritten. */
 FD_API int fd_pages_compact(void* stream, const fd_page_pool* pool, const fd_page_tables* tables, int32_t* live_out,
                             void* workspace, int64_t workspace_bytes);
 

@@ -170,3 +170,21 @@ def test_the_callers_workspace_gives_the_same_lse(fd):
         check(out, lse, *oracle_prefill(q, pg.seq, ql, True, 0.09), BF16, 3000, pg.vmax)
         got.append((out, lse))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]) and not (ws == 255).all()
+
+
+@pytest.mark.parametrize("tokens", [5, 100])
+@pytest.mark.parametrize("cap", [30.0, 512.0, 4096.0])
+def test_soft_caps_of_all_sizes(fd, cap, tokens):
+    """A capped score, cap (1 - 2 / (1 + e^2y)), is off by a few roundings of numbers up to cap: 2^-22 cap, on top of what 32-bit
+    products of large scores are off by (as in the test of sharp scores)."""
+    g = torch.Generator().manual_seed(71)
+    n, m, Hq, Hkv, D, scale, factor = tokens, 400, 4, 2, 128, 0.09, 20.0
+    q = (torch.randn(n, Hq, D, generator=g) * factor).to(BF16)
+    k, v = (torch.randn(m, Hkv, D, generator=g).to(BF16) for _ in range(2))
+    lse = torch.empty(n, Hq, device=DEV)
+    out = fd.gqa_fwd_batch_prefill(q.to(DEV), k.to(DEV), v.to(DEV), starts([n]).to(DEV), None, None, scale, cap,
+                                   cu_seqlens_k=starts([m]).to(DEV), lse_out=lse)
+    ref, ref_lse, mag = oracle_prefill(q, [[k.double()], [v.double()]], [n], True, scale, cap)
+    e = 4 * D * 2.0 ** -24 * scale * 2 * D * factor + 2 * cap * 2.0 ** -22
+    assert ((out.double().cpu() - ref).abs() <= (2.0 ** -8 + 2.0 ** -11 + e) * (mag + ref.abs())).all()
+    assert ((lse.double().cpu() - ref_lse).abs() <= 2.0 ** -12 + e).all()

@@ -764,8 +764,8 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
   };
   // No barrier.  16-bit caches: one block deep per wave, K of the next block is requested when this one's scores are done, V
   // when its product is; the waves of two workgroups cover each other's waits.  fp8: kDeep blocks in registers, a block is
-  // requested as soon as the one kDeep before it is in LDS (own keys of 128 sequences: two deep is level with one, and one
-  // spills nothing).  Page entries are read a block ahead and before that block's requests: loads return in order, and the
+  // requested as soon as the one kDeep before it is in LDS (own keys of 128 sequences: two deep is level with one and needs
+  // more registers).  Page entries are read a block ahead and before that block's requests: loads return in order, and the
   // wait for an entry is one for what came before it.
   auto walk = [&](auto careful_tag) {
     constexpr bool CAREFUL = decltype(careful_tag)::value;
@@ -792,8 +792,8 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
       for (int d = 0; d < kDeep; ++d) request_both(t0 + d * kStep, raw[d]);
       for (; t0 < hi; t0 += kDeep * kStep) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d) {       // (this form also keeps head dim 256 from spilling: 161 -> 92 us a step of
-          const int t = t0 + d * kStep;         // eight sequences of 8000 tokens)
+        for (int d = 0; d < kDeep; ++d) {       // (as a plain loop head dim 256 spills 64 - 120 registers, in this form 17:
+          const int t = t0 + d * kStep;         // 161 -> 92 us a step of eight sequences of 8000 tokens)
           if (t >= hi) break;
           deposit(raw[d]);
           request_both(t + kDeep * kStep, raw[d]);
@@ -863,7 +863,10 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
 }
 
 // T: query and product type.  FP8: e4m3 cache.  CAP: soft-capped scores.  D: head dim.  ROWS: tiles of 128 rows, else of 32.
-// (The bodies keep two workgroups of four waves on a CU: at most 256 registers a wave, 512 with a head dim of 256.)
+// The bodies keep two workgroups of four waves on a CU, one with a head dim of 256: at most 256 registers a lane, 512 there.
+// What does not fit goes to scratch.  Registers spilled (bytes a lane), without and with a soft cap: none with a head dim of
+// 64; key tiles none with 128, 9 and 18 (40, 72) with 256, over fp8 17 and 0 (72, 0); row tiles, whose kernel holds both
+// bodies, 6 and 8 (28, 36) with 128, over fp8 4 and 5 (20, 24), and 23 and 37 (68, 100) with 256, over fp8 43 and 33 (136).
 template <typename T, bool FP8, bool CAP, int D, bool ROWS>
 __global__ void __launch_bounds__(64 * kPrefillWaves, D == 256 ? 1 : 2) fd_prefill_kernel(const PrefillArgs a) {
   extern __shared__ __align__(1024) char smem[];

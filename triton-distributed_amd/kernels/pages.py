@@ -150,7 +150,8 @@ def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Opti
                      stream=None) -> torch.Tensor:
     """Moves the live pages to the front of the pool, in every layer: with ``n`` live pages, the k-th live page at or behind
     ``n`` goes to the k-th free page before ``n``; ``page_refs`` and ``block_table`` follow.  ``block_table`` must hold every
-    row that holds pages.  Returns int32 ``[1]`` (on the device): ``n``, from where on the pool is free."""
+    row that holds pages; page ids kept anywhere else (a ``prefix_table`` that is no part of it) are not rewritten.  Returns
+    int32 ``[1]`` (on the device): ``n``, from where on the pool is free."""
     pool, t = _checked("paged_kv_compact", (k_cache, v_cache), (block_table, None, page_refs), (("live_out", live_out, (1,)),))
     if live_out is None:
         live_out = _new(1, torch.int32, k_cache.device, stream, returned=True)

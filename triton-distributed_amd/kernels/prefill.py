@@ -141,8 +141,9 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
 
     ``causal``: row ``i`` of ``n_q`` sees the keys ``j <= i + n_k - n_q`` -- the last row sees the last key; otherwise all
     rows see all keys of their sequence.  A row that sees nothing gets 0 (LSE ``-inf``); rows that belong to no sequence
-    are left as they are in ``output`` and ``lse_out`` (fp32 ``[total_q, Hq]``, natural log).  Head dims 64, 128, 256,
-    fp16 / bf16, any number of query heads per KV head.
+    are left as they are in ``output`` and ``lse_out`` (fp32 ``[total_q, Hq]``, natural log).  A row that meets a NaN -- its
+    own, a key's that it sees, a scale's -- is NaN, however its keys are split.  ``soft_cap``: 0 is off; a capped score is good
+    to ``soft_cap * 2**-22``.  Head dims 64, 128, 256, fp16 / bf16, any number of query heads per KV head.
 
     ``workspace``: a contiguous GPU tensor on a 256-byte boundary that is used for partials if it is large enough
     (``prefill_workspace_bytes``).  ``max_kv_len``: an upper bound of the key counts, a hint.  ``kv_split``: 0 lets the

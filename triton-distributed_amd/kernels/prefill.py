@@ -51,17 +51,15 @@ def _check_scales(name, k_scale, v_scale, kv_heads):
               f"{name}: fp8 scales are contiguous float32 tensors of {kv_heads} values")
 
 
-def _check_no_grad(name, *tensors):
-    """No argument (queries, keys, values, fp8 scales) that a derivative goes through, in either mode."""
-    backward = torch.is_grad_enabled()
-    forward = getattr(forward_ad, "_current_level", 0) >= 0     # (outside every dual level nothing carries a tangent)
-    if backward or forward:
-        for t in tensors:
-            if t is None:
-                continue
-            if backward and t.requires_grad:
-                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
-            if forward and forward_ad.unpack_dual(t).tangent is not None:
+def _check_no_grad(name, q, k, v, k_scale, v_scale):
+    """No argument that a derivative goes through, in either mode."""
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or k_scale is not None and k_scale.requires_grad
+                                    or v_scale is not None and v_scale.requires_grad):
+        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or inference_mode()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:      # (outside every dual level nothing carries a tangent)
+        for t in (q, k, v, k_scale, v_scale):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise RuntimeError(f"{name} has no forward-mode derivative: an argument carries a tangent")
 
 
@@ -85,7 +83,8 @@ def _check_table(name, what, table, rows):
 
 def _launch(fn, device, stream, *args):
     """Calls the library on the tensors' device, whatever the current one is, and raises what it reports."""
-    _need(stream is None or stream.device == device, f"tensors on {device}, a stream of another device")
+    if stream is not None and stream.device != device:
+        raise RuntimeError(f"tensors on {device}, a stream of another device")
     if device.index == torch.cuda.current_device():
         rc = fn(stream_handle(stream, device.index), *args)
     else:
@@ -272,7 +271,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache, k_scale, v_scale)
     scale, soft_cap = float(scale), float(soft_cap or 0.0)
     # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
-    hints = tuple(-(-int(n or 0) // 1024) * 1024 for n in (max_kv_len, max_prefix_len))
+    hints = (-(-int(max_kv_len or 0) // 1024) * 1024, -(-int(max_prefix_len or 0) // 1024) * 1024)
     key = (_sig(q), _sig(k_cache), _sig(v_cache), _sig(kv_lens), _sig(block_table), _sig(prefix_lens), _sig(prefix_table),
            _sig(group_starts), _sig(output_combine), _sig(lse_out), _sig(k_scale), _sig(v_scale), scale, soft_cap, hints)
     cached = _SHARED_CACHE.get(key)

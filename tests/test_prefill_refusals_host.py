@@ -28,6 +28,9 @@ def test_prefill_keywords_are_refused_before_the_append(fd):
     for name in ("output", "cu_seqlens_k", "k_scale", "no_such_keyword"):
         with pytest.raises(TypeError, match="unexpected keyword " + name):
             attn.prefill(torch.zeros(2, 3, 8), None, None, None, 0, **{name: 1})
+    for bad in (torch.zeros(2, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32)):
+        with pytest.raises(RuntimeError, match="q_lens must be int32"):
+            attn.prefill(torch.zeros(2, 3, 8), None, None, None, 0, q_lens=bad)
 
 
 def test_arguments_with_derivatives(fd):

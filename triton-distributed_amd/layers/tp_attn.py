@@ -124,6 +124,8 @@ class TP_Attn:
         if unknown:      # (before anything is appended)
             raise TypeError(f"TP_Attn.prefill: unexpected keyword {unknown[0]}")
         bsz, q_len, _ = x.size()
+        if q_lens is not None and (q_lens.dtype != torch.int32 or tuple(q_lens.shape) != (bsz,)):
+            raise RuntimeError(f"TP_Attn.prefill: q_lens must be int32 of shape ({bsz},), got {q_lens.dtype} {tuple(q_lens.shape)}")
         if q_len == 0:
             return x.new_empty(bsz, 0, self.wo.shape[0])
         qkv = nn.functional.linear(x, self.wqkv)

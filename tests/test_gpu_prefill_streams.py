@@ -110,6 +110,7 @@ def test_the_cached_attention_call(fd, shared):
                                torch.arange(B * 32, B * 32 + 7, dtype=torch.int32, device=DEV).view(1, 7), None)
     got = []
     for on_side in (False, True, True):
+        kw["cache_seqlens"] = lens.view(B, 1) if got else lens      # (as many numbers as sequences, in any shape)
         kc, vc = (p.clone() for p in pools)
         side = side_stream()
         if on_side:

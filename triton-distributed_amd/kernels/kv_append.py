@@ -293,8 +293,8 @@ def flash_attn_with_kvcache(q, k_cache, v_cache, k=None, v=None, rotary_cos=None
     lse = torch.empty((bsz, q_heads), dtype=torch.float32, device=dev) if return_softmax_lse else None
     if shared_prefix is not None:
         prefix_lens, prefix_table, group_starts = shared_prefix
-        gqa_fwd_batch_decode_shared_prefix(q_rot[:, 0], k_cache, v_cache, None, None, kv_lens, block_table, prefix_lens,
-                                           prefix_table, scale, softcap, group_starts=group_starts,
+        gqa_fwd_batch_decode_shared_prefix(q_rot[:, 0], k_cache, v_cache, None, None, kv_lens.reshape(bsz), block_table,
+                                           prefix_lens, prefix_table, scale, softcap, group_starts=group_starts,
                                            output_combine=out[:, 0], lse_out=lse, k_scale=k_scale, v_scale=v_scale,
                                            **decode_kw)
         return (out, lse.view(bsz, q_heads, 1)) if return_softmax_lse else out

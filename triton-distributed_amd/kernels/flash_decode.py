@@ -53,6 +53,7 @@ use).
 """
 from __future__ import annotations
 
+import functools
 from ctypes import addressof, byref
 from typing import Optional
 
@@ -102,26 +103,51 @@ def _require_cuda(*tensors):
             raise RuntimeError("flash-decode tensors must live on the GPU; this package has no CPU path")
 
 
-def _new(shape, dtype, device, stream, returned=False):
-    """A new tensor for work on ``stream`` (None: the current one).  It comes from that stream's pool: a block of the current
-    stream's may still be in use by work that is queued there.  ``returned``: the caller may use it on the current stream."""
+def _on(stream, fn, *args, **kw):
+    """``fn(*args, **kw)``, all of its work and the memory it takes, on ``stream`` instead of the current one (None: there).
+    Memory of the current stream's pool may still be in use by work that is queued there."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        t = torch.empty(shape, dtype=dtype, device=device)
-    if returned:
-        t.record_stream(torch.cuda.current_stream(device))
-    return t
+        return fn(*args, **kw)
+    device = stream.device
+    for t in args:
+        if isinstance(t, torch.Tensor):
+            if t.is_cuda and t.device != device:
+                raise RuntimeError(f"{fn.__name__}: tensors on {t.device}, a stream of {device}")
+            break
+    if stream.cuda_stream == stream_handle(None, device.index):
+        return fn(*args, **kw)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _on(stream, fn, *args, **kw)
+    current = torch.cuda.current_stream()
+    torch.cuda.set_stream(stream)              # (a third of what the context manager costs)
+    try:
+        out = fn(*args, **kw)
+    finally:
+        torch.cuda.set_stream(current)
+    for t in out if isinstance(out, tuple) else (out,):
+        if isinstance(t, torch.Tensor):
+            t.record_stream(current)           # (the caller uses it there)
+    return out
 
 
-def schedule_sequences(kv_lens: torch.Tensor, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+def _on_stream(fn):
+    """``fn`` with ``stream=``: the caller orders the stream behind what the arguments need, and what uses the result behind it."""
+    @functools.wraps(fn)
+    def call(*args, stream=None, **kw):
+        return fn(*args, **kw) if stream is None else _on(stream, fn, *args, **kw)
+    return call
+
+
+@_on_stream
+def schedule_sequences(kv_lens: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Kernel (3): int32 [B] sequence order, longest kv_len first, computed on the device."""
     _require_cuda(kv_lens)
     lib = load_library()
     assert kv_lens.dtype == torch.int32 and kv_lens.is_contiguous()
     if out is None:
-        out = _new(kv_lens.shape, torch.int32, kv_lens.device, stream, returned=True)
-    check(lib.fd_schedule(stream_handle(stream, kv_lens.device.index), kv_lens.data_ptr(), kv_lens.numel(),
+        out = torch.empty_like(kv_lens)
+    check(lib.fd_schedule(stream_handle(None, kv_lens.device.index), kv_lens.data_ptr(), kv_lens.numel(),
                           out.data_ptr()))
     return out
 
@@ -245,7 +271,7 @@ _STEP_CACHE = {}   # fd_decode_args images of planned steps by everything but th
 
 def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine,
             kv_split, *, with_lse_column: bool, lse_out=None, k_scale=None, v_scale=None, extra_partials=None, seq_order=None,
-            seq_order_lens=None, stream=None, path="auto", waves_per_block=0, fuse_combine=False, plan_splits=True,
+            seq_order_lens=None, path="auto", waves_per_block=0, fuse_combine=False, plan_splits=True,
             schedule_items=False, item_order=None, max_kv_len=None, no_alloc=False, auto_order=True, rank_merge=None,
             _prepare=False):
     batch, q_heads, q_head_dim = q.shape
@@ -267,7 +293,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
     if output_combine is None:
         if no_alloc:
             raise RuntimeError("no_alloc=True needs output_combine")
-        output_combine = _new([batch, q_heads, out_cols], q.dtype, q.device, stream, returned=True)
+        output_combine = torch.empty([batch, q_heads, out_cols], dtype=q.dtype, device=q.device)
     else:
         _require_cuda(output_combine)
     oc_st = output_combine.stride()
@@ -302,7 +328,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
         assert seq_order is not None and seq_order_lens.dtype == torch.int32 and seq_order_lens.is_contiguous()
         assert seq_order_lens.numel() == batch
     lib = load_library()
-    hstream = stream.cuda_stream if stream is not None else stream_handle(None, q.device.index)
+    hstream = stream_handle(None, q.device.index)
     flags = ((0 if plan_splits else FD_STEP_EXACT_SPLITS) | (FD_STEP_SCHEDULE if schedule_items else 0)
              | (0 if auto_order else FD_STEP_NO_ORDER))
 
@@ -341,7 +367,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
                 and workspace.numel() * workspace.element_size() >= need):
             hold = workspace     # the caller's workspace is large enough: no allocation in the call
         else:
-            hold = _new(need, torch.uint8, q.device, stream)
+            hold = torch.empty(need, dtype=torch.uint8, device=q.device)
         a.q, a.k_cache, a.v_cache = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
         a.workspace, a.workspace_bytes = hold.data_ptr(), need
         a.out, a.block_table, a.kv_lens = output_combine.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr()
@@ -407,13 +433,13 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
                 and workspace.is_contiguous() and workspace.numel() >= n_o + n_l):
             hold = workspace
         else:
-            hold = _new(n_o + n_l, torch.float32, q.device, stream)
+            hold = torch.empty(n_o + n_l, dtype=torch.float32, device=q.device)
         mid_ptr = hold.data_ptr() if hold is not None else None
         lse_split_ptr = mid_ptr + 4 * n_o if hold is not None else None
         so_b, so_h, so_s = q_heads * num_splits * v_head_dim, num_splits * v_head_dim, v_head_dim
     want_items = (item_order is not None and num_splits > 1 and not fuse_combine) or plan.order_kind == FD_ORDER_ITEMS
     if plan.order_kind == FD_ORDER_SEQUENCES:
-        seq_order = schedule_sequences(kv_lens, stream=stream)
+        seq_order = schedule_sequences(kv_lens)
     p = _make_params(q, k_cache, block_table, num_splits, soft_cap, plan.mid_dtype, out_dtype, k_scale, v_scale, path,
                      waves_per_block, seq_order_lens, plan.split_align, plan.split_adapt, 0, plan.max_kv_len, v_head_dim)
     if want_items:
@@ -421,7 +447,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
         # it) or computed here by one scheduling launch.  With the caller's exact split count the items are the
         # reference's ranges (every slot of the partial buffer is still written, empty ranges last).
         if item_order is None:
-            item_order = _new(2 * batch * num_splits, torch.int32, q.device, stream)
+            item_order = item_order_buffer(batch, num_splits, q.device)
             check(lib.fd_schedule_items(hstream, kv_lens.data_ptr(), batch, item_order.data_ptr(), byref(p)))
         assert item_order.dtype == torch.int32 and item_order.is_contiguous()
         assert item_order.numel() >= 2 * batch * num_splits
@@ -439,7 +465,7 @@ def _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_ca
             oc_st[0], oc_st[1], seq_order.data_ptr() if seq_order is not None else None, mode,
             ex_out.data_ptr() if n_extra else None, ex_lse.data_ptr() if n_extra else None, n_extra, byref(p)))
         return output_combine
-    tickets = _tickets(q.device, hstream, batch * q_heads, stream) if fuse_combine else None
+    tickets = _tickets(q.device, hstream, batch * q_heads) if fuse_combine else None
     check(lib.fd_decode(
         hstream, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), mid_ptr, lse_split_ptr,
         output_combine.data_ptr(), lse_out.data_ptr() if lse_out is not None else None, float(scale),
@@ -482,13 +508,13 @@ class PreparedDecode:
             kw["schedule_items"] = True
         cols = v_cache.shape[-1] + (1 if variant == "intra_rank" else 0)
         if output_combine is None:
-            output_combine = _new((q.shape[0], q.shape[1], cols), q.dtype, q.device, stream, returned=True)
+            output_combine = _on(stream, torch.empty, (q.shape[0], q.shape[1], cols), dtype=q.dtype, device=q.device)
         self._lib = load_library()
         self._stream = stream
         self._device = q.device.index
-        self._args, self._keep = _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, None,
-                                         output_combine, kv_split, with_lse_column=variant == "intra_rank",
-                                         stream=stream, _prepare=True, **kw)
+        self._args, self._keep = _on(stream, _decode, q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap,
+                                     None, output_combine, kv_split, with_lse_column=variant == "intra_rank",
+                                     _prepare=True, **kw)
         self._ref = byref(self._args)
         self._tensors = dict(q=q, k_cache=k_cache, v_cache=v_cache, kv_lens=kv_lens, block_table=block_table,
                              output_combine=output_combine, lse_out=kw.get("lse_out"), kw=kw)
@@ -520,14 +546,21 @@ _PLAN_CACHE = {}   # fd_plan_decode results by problem shape
 _TICKETS = {}
 
 
-def _tickets(device, hstream, n, stream):
+def _tickets(device, hstream, n):
     key = (device.index, hstream)
     t = _TICKETS.get(key)
     if t is None or t.numel() < n:
-        t = _TICKETS[key] = _new(max(n, 4096), torch.int32, device, stream)
-        with torch.cuda.stream(stream):      # (None: the current one)
-            t.zero_()
+        t = torch.zeros(max(n, 4096), dtype=torch.int32, device=device)
+        _TICKETS[key] = t
     return t
+
+
+def _step(kw):
+    """``_decode``, on the stream that the keywords name if it is not the current one anyway."""
+    stream = kw.pop("stream", None)
+    if stream is None or stream.cuda_stream == stream_handle(None, stream.device_index):
+        return _decode
+    return functools.partial(_on, stream, _decode)
 
 
 def gqa_fwd_batch_decode(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, scale, soft_cap=0.0,
@@ -540,16 +573,16 @@ def gqa_fwd_batch_decode(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_
     ``kv_lens`` that the caller knows on the host; the launch shape is then planned for it instead of for the block
     table's capacity (a hint only: longer sequences are still decoded in full).
     """
-    return _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
-                   with_lse_column=False, **kw)
+    return _step(kw)(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
+                     with_lse_column=False, **kw)
 
 
 def gqa_fwd_batch_decode_intra_rank(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, scale,
                                     soft_cap=0.0, output_split=None, output_combine=None, kv_split=-1, **kw):
     """Split-KV decode + combine that also stores the merged LSE at column Dv:
     ``output_combine [B, Hq, Dv+1]`` (flash_decode.py:847-928)."""
-    return _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
-                   with_lse_column=True, **kw)
+    return _step(kw)(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
+                     with_lse_column=True, **kw)
 
 
 def gqa_fwd_batch_decode_persistent(q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, scale, soft_cap=0,
@@ -560,8 +593,8 @@ def gqa_fwd_batch_decode_persistent(q, k_cache, v_cache, workspace, q_lens, kv_l
     workgroups over the CUs, so no co-residency assumption is needed."""
     if kw.get("seq_order") is None and kw.get("item_order") is None and q.shape[0] > 1:
         kw["schedule_items"] = True   # a single sequence has nothing to order
-    return _decode(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
-                   with_lse_column=False, **kw)
+    return _step(kw)(q, k_cache, v_cache, workspace, kv_lens, block_table, scale, soft_cap, output_split, output_combine, kv_split,
+                     with_lse_column=False, **kw)
 
 
 def gqa_fwd_batch_decode_aot(stream, q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table, scale, soft_cap=0,

@@ -14,7 +14,6 @@ Every function enqueues hand-written HIP kernels through the C ABI in
 """
 from __future__ import annotations
 
-import functools
 from ctypes import byref
 from typing import Optional, Tuple, Union
 
@@ -23,7 +22,7 @@ import torch
 from .._lib import FdParams, FdQkPrep, check, fd_dtype_of, load_library, stream_handle
 from .._lib import (FD_ORDER_ITEMS, FD_ORDER_SEQUENCES, FD_STEP_EXACT_SPLITS, FD_STEP_FUSED,
                     FD_STEP_ORDER_FROM_APPEND)
-from .flash_decode import _decode, _require_cuda, decode_plan, item_order_buffer
+from .flash_decode import _decode, _on_stream, _require_cuda, decode_plan, item_order_buffer
 from .prefill import gqa_fwd_batch_decode_shared_prefix
 
 
@@ -46,22 +45,6 @@ def _prep_struct(cos_sin, position_ids, head_dim, bsz, seq) -> FdQkPrep:
     r.max_positions = cos_sin.shape[0]
     r.stride_pos_b, r.stride_pos_t = position_ids.stride(0), position_ids.stride(1)
     return r
-
-
-def _on_stream(fn):
-    """``fn`` with ``stream=``: all of its work, and what it allocates, on that stream; the caller orders the stream behind
-    what the arguments need and what uses the result behind it."""
-    @functools.wraps(fn)
-    def call(*args, stream=None, **kw):
-        if stream is None:
-            return fn(*args, **kw)
-        with torch.cuda.stream(stream):
-            out = fn(*args, **kw)
-        for t in out if isinstance(out, tuple) else (out,):
-            if t is not None:
-                t.record_stream(torch.cuda.current_stream(t.device))   # (the caller uses it there)
-        return out
-    return call
 
 
 @_on_stream

@@ -21,7 +21,8 @@ from typing import Optional, Union
 import torch
 
 from .._lib import FdPagePool, FdPageTables, load_library
-from .prefill import _check_devices, _check_int32, _launch, _need, _new, _remember, _sig
+from .flash_decode import _on
+from .prefill import _check_devices, _check_int32, _launch, _need, _remember, _sig
 
 
 def _pool(name, k_cache, v_cache) -> FdPagePool:
@@ -88,10 +89,12 @@ def _checked(name, caches, tables, lists):
 def paged_kv_copy(k_cache, v_cache, src_pages, dst_pages, *, stream=None):
     """Copies page ``src_pages[i]`` to page ``dst_pages[i]`` (int32 ``[n]``) in every layer of both pools.  The destinations
     must be distinct and none of them a source; ids outside the pool are skipped."""
+    if stream is not None:
+        return _on(stream, paged_kv_copy, k_cache, v_cache, src_pages, dst_pages)
     n = src_pages.numel()
     pool, _ = _checked("paged_kv_copy", (k_cache, v_cache), (), (("src_pages", src_pages, (n,)), ("dst_pages", dst_pages, (n,))))
     if n:
-        _launch(load_library().fd_pages_copy, k_cache.device, stream, byref(pool), src_pages.data_ptr(), dst_pages.data_ptr(), n)
+        _launch(load_library().fd_pages_copy, k_cache.device, byref(pool), src_pages.data_ptr(), dst_pages.data_ptr(), n)
 
 
 def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, torch.Tensor], page_size: int, *,
@@ -101,16 +104,18 @@ def paged_kv_reserve(block_table, kv_lens, page_refs, new_tokens: Union[int, tor
     run out, or the row wants tokens but lacks a page for those that its length counts already (its length went up
     without pages: free it first) -- that row keeps what it had.  Rows are served in order; a row that gets nothing for want of
     free pages still counts against the rows behind it.  At most 4096 rows, and 2^20 new pages a row."""
+    if stream is not None:
+        return _on(stream, paged_kv_reserve, block_table, kv_lens, page_refs, new_tokens, page_size, ok_out=ok_out)
     each = new_tokens if isinstance(new_tokens, torch.Tensor) else None
     batch = block_table.shape[0]
     _, t = _checked("paged_kv_reserve", (), (block_table, kv_lens, page_refs),
                     (("new_tokens", each, (batch,)), ("ok_out", ok_out, (batch,))))
     if ok_out is None:
-        ok_out = _new(batch, torch.int32, block_table.device, stream, returned=True)
+        ok_out = torch.empty(batch, dtype=torch.int32, device=block_table.device)
     _need(batch <= 4096, f"paged_kv_reserve: {batch} rows (at most 4096)")
     _need(each is not None or 0 <= new_tokens < 1 << 31, f"paged_kv_reserve: new_tokens {new_tokens}")
     if batch:
-        _launch(load_library().fd_pages_reserve, block_table.device, stream, byref(t), page_refs.numel(), int(page_size),
+        _launch(load_library().fd_pages_reserve, block_table.device, byref(t), page_refs.numel(), int(page_size),
                 each.data_ptr() if each is not None else None, 0 if each is not None else int(new_tokens), ok_out.data_ptr())
     return ok_out
 
@@ -123,16 +128,18 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
     parent, a parent without a page for tokens that its length counts, a child that holds tokens or pages or was named
     before, no free page left).  Parents count as they are before
     the call.  At most 16384 forks."""
+    if stream is not None:
+        return _on(stream, paged_kv_fork, k_cache, v_cache, block_table, kv_lens, page_refs, parents, children, ok_out=ok_out)
     n = parents.numel()
     pool, t = _checked("paged_kv_fork", (k_cache, v_cache), (block_table, kv_lens, page_refs),
                        (("parents", parents, (n,)), ("children", children, (n,)), ("ok_out", ok_out, (n,))))
     if ok_out is None:
-        ok_out = _new(n, torch.int32, k_cache.device, stream, returned=True)
+        ok_out = torch.empty(n, dtype=torch.int32, device=k_cache.device)
     if n:
         lib = load_library()
         need = lib.fd_pages_workspace_bytes(pool.num_pages, n)
-        ws = _new(need, torch.uint8, k_cache.device, stream)
-        _launch(lib.fd_pages_fork, k_cache.device, stream, byref(pool), byref(t), parents.data_ptr(), children.data_ptr(), n,
+        ws = torch.empty(need, dtype=torch.uint8, device=k_cache.device)
+        _launch(lib.fd_pages_fork, k_cache.device, byref(pool), byref(t), parents.data_ptr(), children.data_ptr(), n,
                 ok_out.data_ptr(), ws.data_ptr(), need)
     return ok_out
 
@@ -140,10 +147,12 @@ def paged_kv_fork(k_cache, v_cache, block_table, kv_lens, page_refs, parents, ch
 def paged_kv_free(block_table, kv_lens, page_refs, rows, *, stream=None):
     """Takes their pages from the listed rows (int32 ``[n]``): counts go down -- a page that no row holds any more is free --,
     the rows' entries become -1 and their lengths 0.  Empty rows, rows listed twice and rows out of range are skipped."""
+    if stream is not None:
+        return _on(stream, paged_kv_free, block_table, kv_lens, page_refs, rows)
     n = rows.numel()
     _, t = _checked("paged_kv_free", (), (block_table, kv_lens, page_refs), (("rows", rows, (n,)),))
     if n and t.batch:
-        _launch(load_library().fd_pages_free, block_table.device, stream, byref(t), page_refs.numel(), rows.data_ptr(), n)
+        _launch(load_library().fd_pages_free, block_table.device, byref(t), page_refs.numel(), rows.data_ptr(), n)
 
 
 def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Optional[torch.Tensor] = None,
@@ -152,11 +161,13 @@ def paged_kv_compact(k_cache, v_cache, block_table, page_refs, *, live_out: Opti
     ``n`` goes to the k-th free page before ``n``; ``page_refs`` and ``block_table`` follow.  ``block_table`` must hold every
     row that holds pages; page ids kept anywhere else (a ``prefix_table`` that is no part of it) are not rewritten.  Returns
     int32 ``[1]`` (on the device): ``n``, from where on the pool is free."""
+    if stream is not None:
+        return _on(stream, paged_kv_compact, k_cache, v_cache, block_table, page_refs, live_out=live_out)
     pool, t = _checked("paged_kv_compact", (k_cache, v_cache), (block_table, None, page_refs), (("live_out", live_out, (1,)),))
     if live_out is None:
-        live_out = _new(1, torch.int32, k_cache.device, stream, returned=True)
+        live_out = torch.empty(1, dtype=torch.int32, device=k_cache.device)
     lib = load_library()
     need = lib.fd_pages_workspace_bytes(pool.num_pages, 0)
-    ws = _new(need, torch.uint8, k_cache.device, stream)
-    _launch(lib.fd_pages_compact, k_cache.device, stream, byref(pool), byref(t), live_out.data_ptr(), ws.data_ptr(), need)
+    ws = torch.empty(need, dtype=torch.uint8, device=k_cache.device)
+    _launch(lib.fd_pages_compact, k_cache.device, byref(pool), byref(t), live_out.data_ptr(), ws.data_ptr(), need)
     return live_out

@@ -24,7 +24,7 @@ from torch.autograd import forward_ad
 
 from .._lib import (FD_COMBINE_SPLIT, FdParams, FdPrefillArgs, FdSharedArgs, check, fd_dtype_of, load_library,
                     stream_handle)
-from .flash_decode import _new, _require_cuda
+from .flash_decode import _on, _require_cuda
 
 
 def _need(condition, message):
@@ -81,15 +81,13 @@ def _check_table(name, what, table, rows):
           f"{name}: {what} must be int32 [{rows}, max_pages] with contiguous rows, got {table.dtype} {tuple(table.shape)}")
 
 
-def _launch(fn, device, stream, *args):
+def _launch(fn, device, *args):
     """Calls the library on the tensors' device, whatever the current one is, and raises what it reports."""
-    if stream is not None and stream.device != device:
-        raise RuntimeError(f"tensors on {device}, a stream of another device")
     if device.index == torch.cuda.current_device():
-        rc = fn(stream_handle(stream, device.index), *args)
+        rc = fn(stream_handle(None, device.index), *args)
     else:
         with torch.cuda.device(device):
-            rc = fn(stream_handle(stream, device.index), *args)
+            rc = fn(stream_handle(None, device.index), *args)
     if rc:
         check(rc)
 
@@ -99,14 +97,14 @@ def _sig(t):
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-def _workspace(workspace, need, device, stream):
+def _workspace(workspace, need, device):
     """The caller's workspace if it is large enough and aligned, else a new one."""
     if not need:
         return None
     if (isinstance(workspace, torch.Tensor) and workspace.device == device and workspace.is_contiguous()
             and workspace.data_ptr() % 256 == 0 and workspace.numel() * workspace.element_size() >= need):
         return workspace
-    return _new(need, torch.uint8, device, stream)
+    return torch.empty(need, dtype=torch.uint8, device=device)
 
 
 _PREFILL_CACHE = {}   # fd_prefill_args images of calls by everything but the pointers
@@ -149,6 +147,10 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     library choose how many key ranges a row tile is cut into (more than one where there are few rows), else exactly that
     many, up to 64.
     """
+    if stream is not None:
+        return _on(stream, gqa_fwd_batch_prefill, q, k, v, cu_seqlens_q, kv_lens, block_table, scale, soft_cap, causal=causal,
+                   cu_seqlens_k=cu_seqlens_k, q_lens=q_lens, output=output, lse_out=lse_out, k_scale=k_scale, v_scale=v_scale,
+                   workspace=workspace, max_kv_len=max_kv_len, kv_split=kv_split)
     _check_no_grad("gqa_fwd_batch_prefill", q, k, v, k_scale, v_scale)
     # (values: a tensor could change under the key)
     scale, soft_cap, causal = float(scale), float(soft_cap or 0.0), bool(causal)
@@ -162,7 +164,7 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
             q_lens, output, lse_out, k_scale, v_scale, max_kv_len, kv_split))
     image, need = cached
     if output is None:
-        output = _new(q.shape, q.dtype, q.device, stream, returned=True)
+        output = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if image is None:      # no rows, or no sequence
         return output
     a = FdPrefillArgs.from_buffer_copy(image)
@@ -181,9 +183,9 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     if k_scale is not None:
         a.params.k_scale, a.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
     if need:
-        hold = _workspace(workspace, need, q.device, stream)
+        hold = _workspace(workspace, need, q.device)
         a.workspace, a.workspace_bytes = hold.data_ptr(), need
-    _launch(load_library().fd_prefill, q.device, stream, byref(a))
+    _launch(load_library().fd_prefill, q.device, byref(a))
     return output
 
 
@@ -268,6 +270,10 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
     group's query heads.  ``q_lens`` is accepted and ignored, ``workspace`` used if it is large enough, as there; 16-bit
     queries with a cache of the same type or fp8-e4m3.  ``max_kv_len`` / ``max_prefix_len``: host-side hints.
     """
+    if stream is not None:
+        return _on(stream, gqa_fwd_batch_decode_shared_prefix, q, k_cache, v_cache, workspace, q_lens, kv_lens, block_table,
+                   prefix_lens, prefix_table, scale, soft_cap, group_starts=group_starts, output_combine=output_combine,
+                   lse_out=lse_out, k_scale=k_scale, v_scale=v_scale, max_kv_len=max_kv_len, max_prefix_len=max_prefix_len)
     _check_no_grad("gqa_fwd_batch_decode_shared_prefix", q, k_cache, v_cache, k_scale, v_scale)
     scale, soft_cap = float(scale), float(soft_cap or 0.0)
     # (the length hints count in steps of 1024 tokens, so that a growing batch keeps its prepared step)
@@ -281,12 +287,12 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
             soft_cap, group_starts, output_combine, lse_out, k_scale, v_scale, hints))
     image, need = cached
     if output_combine is None:
-        output_combine = _new(q.shape, q.dtype, q.device, stream, returned=True)
+        output_combine = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if image is None:      # no sequence
         return output_combine
     a = FdSharedArgs.from_buffer_copy(image)
     s = a.step
-    hold = _workspace(workspace, need, q.device, stream)
+    hold = _workspace(workspace, need, q.device)
     s.workspace, s.workspace_bytes = hold.data_ptr(), need
     s.q, s.k_cache, s.v_cache, s.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), output_combine.data_ptr()
     s.block_table, s.kv_lens = block_table.data_ptr(), kv_lens.data_ptr()
@@ -297,7 +303,7 @@ def gqa_fwd_batch_decode_shared_prefix(q, k_cache, v_cache, workspace, q_lens, k
         s.lse_out = lse_out.data_ptr()
     if k_scale is not None:
         s.params.k_scale, s.params.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
-    _launch(load_library().fd_decode_shared, q.device, stream, byref(a))
+    _launch(load_library().fd_decode_shared, q.device, byref(a))
     return output_combine
 
 

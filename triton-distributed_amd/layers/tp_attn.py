@@ -19,7 +19,8 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ..kernels.kv_append import _dense_block_table, _on_stream, flash_attn_with_kvcache, rope_kv_append
+from ..kernels.flash_decode import _on_stream
+from ..kernels.kv_append import _dense_block_table, flash_attn_with_kvcache, rope_kv_append
 from ..kernels.prefill import gqa_fwd_batch_prefill
 
 

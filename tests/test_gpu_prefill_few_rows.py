@@ -188,3 +188,28 @@ def test_soft_caps_of_all_sizes(fd, cap, tokens):
     e = 4 * D * 2.0 ** -24 * scale * 2 * D * factor + 2 * cap * 2.0 ** -22
     assert ((out.double().cpu() - ref).abs() <= (2.0 ** -8 + 2.0 ** -11 + e) * (mag + ref.abs())).all()
     assert ((lse.double().cpu() - ref_lse).abs() <= 2.0 ** -12 + e).all()
+
+
+@pytest.mark.parametrize("batch", [65, 257, 1025, 2100])
+@pytest.mark.parametrize("paged", [True, False])
+def test_hundreds_and_thousands_of_sequences(fd, batch, paged):
+    """Every row tile finds its sequence among all of them, empty ones and runs of empty ones included."""
+    g = torch.Generator().manual_seed(batch)
+    ql = torch.randint(0, 4, (batch,), generator=g).tolist()
+    ql[batch // 3:batch // 2] = [0] * (batch // 2 - batch // 3)
+    ql[-1] = 40
+    kl = [n + int(e) for n, e in zip(ql, torch.randint(0, 30, (batch,), generator=g))]
+    q = torch.randn(sum(ql), 2, 64, generator=g).to(BF16)
+    lse = torch.empty(sum(ql), 2, device=DEV)
+    if paged:
+        pg = Paged(kl, 1, 64, 16, BF16, seed=5)
+        seqs, vmax = pg.seq, pg.vmax
+        out = fd.gqa_fwd_batch_prefill(q.to(DEV), pg.k, pg.v, starts(ql).to(DEV), pg.lens.to(DEV), pg.table.to(DEV), 0.125,
+                                       lse_out=lse)
+    else:
+        seqs = [[torch.randn(n, 1, 64, generator=g).to(BF16) for n in kl] for _ in range(2)]
+        k, v = (torch.cat(s).to(DEV) for s in seqs)
+        seqs, vmax = [[x.double() for x in s] for s in seqs], 6.0
+        out = fd.gqa_fwd_batch_prefill(q.to(DEV), k, v, starts(ql).to(DEV), None, None, 0.125,
+                                       cu_seqlens_k=starts(kl).to(DEV), lse_out=lse)
+    check(out, lse, *oracle_prefill(q, seqs, ql, True, 0.125), BF16, 100, vmax)

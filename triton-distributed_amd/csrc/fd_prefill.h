@@ -155,6 +155,28 @@ __device__ __forceinline__ int fd_tiles_before(int keys, int tiles, int n, int* 
   return before;
 }
 
+// Steps over blocks of 64 K sequences from b0 on that end before row tile `tile` of the list; `base`: the tiles before b0.
+template <int K>
+__device__ __forceinline__ void fd_skip_sequences(const PrefillArgs& a, int bm, int tile, int& b0, int& base) {
+  const int lane = threadIdx.x & 63;
+  while (b0 < a.batch) {
+    int total = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int b = b0 + lane * K + k;
+      int start, count = 0;
+      if (b < a.batch) fd_prefill_span(a, b, start, count);
+      total += (count * a.G + bm - 1) / bm;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off);
+    total = __builtin_amdgcn_readfirstlane(total);
+    if (tile - base < total) return;
+    base += total;
+    b0 += 64 * K;
+  }
+}
+
 // The lane whose `keys` (at most `top`) are the rank-th largest of the wave's, equal ones in the order of their lanes: the
 // value bit by bit from above, then the lane among those that hold it.
 __device__ __forceinline__ int fd_lane_of_rank(int keys, int rank, int top) {
@@ -220,8 +242,15 @@ __device__ __forceinline__ bool fd_find_item(const PrefillArgs& a, int bm, Prefi
   it.causal = a.causal;
   const int tile = unit / it.splits;
   // The row tile of the list: sequences with the most keys first (in blocks of 64 sequences, one a lane), the tiles of a
-  // sequence from its end, where a causal row sees the most -- short work fills in behind long.
-  for (int b0 = 0, base = 0; b0 < a.batch; b0 += 64) {
+  // sequence from its end, where a causal row sees the most -- short work fills in behind long.  Every workgroup looks for its
+  // own: large batches are stepped through in blocks of 512 and 64 (one token on each of 512 / 5000 caches of up to 400
+  // tokens, 32/8 heads of 128: 328 us / 21.7 ms with the loop over a block's lanes below in every block, 151 us / 1.9 ms).
+  int b0 = 0, base = 0;
+  if (a.batch > 64) {
+    fd_skip_sequences<8>(a, bm, tile, b0, base);
+    fd_skip_sequences<1>(a, bm, tile, b0, base);
+  }
+  for (; b0 < a.batch; b0 += 64) {
     const int mine = b0 + lane;
     int qs = 0, nq = 0, ks = 0, nk = -1, length = 0, tiles = 0;
     if (mine < a.batch) {
@@ -866,7 +895,7 @@ __device__ __forceinline__ void fd_key_tile(const PrefillArgs& a, const PrefillI
 // The bodies keep two workgroups of four waves on a CU, one with a head dim of 256: at most 256 registers a lane, 512 there.
 // What does not fit goes to scratch.  Registers spilled (bytes a lane), without and with a soft cap: none with a head dim of
 // 64; key tiles none with 128, 9 and 18 (40, 72) with 256, over fp8 17 and 0 (72, 0); row tiles, whose kernel holds both
-// bodies, 6 and 8 (28, 36) with 128, over fp8 4 and 5 (20, 24), and 23 and 37 (68, 100) with 256, over fp8 43 and 33 (136).
+// bodies, 6 and 8 (28, 36) with 128, over fp8 4 and 8 (20, 36), and 25 and 37 (76, 104) with 256, over fp8 43 and 32 (136, 124).
 template <typename T, bool FP8, bool CAP, int D, bool ROWS>
 __global__ void __launch_bounds__(64 * kPrefillWaves, D == 256 ? 1 : 2) fd_prefill_kernel(const PrefillArgs a) {
   extern __shared__ __align__(1024) char smem[];

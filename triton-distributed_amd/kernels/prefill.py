@@ -145,7 +145,8 @@ def gqa_fwd_batch_prefill(q, k, v, cu_seqlens_q, kv_lens, block_table, scale, so
     ``workspace``: a contiguous GPU tensor on a 256-byte boundary that is used for partials if it is large enough
     (``prefill_workspace_bytes``).  ``max_kv_len``: an upper bound of the key counts, a hint.  ``kv_split``: 0 lets the
     library choose how many key ranges a row tile is cut into (more than one where there are few rows), else exactly that
-    many, up to 64.
+    many, up to 64.  It chooses for caches of about equal length; for a few long ones among many short ones 8 is better (five
+    drafted tokens on 24 caches of 17 - 16384 tokens: 98 us against 214).
     """
     if stream is not None:
         return _on(stream, gqa_fwd_batch_prefill, q, k, v, cu_seqlens_q, kv_lens, block_table, scale, soft_cap, causal=causal,
